@@ -14,7 +14,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmtts_hip.so")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wno-unused-result",
-         "-ffp-contract=fast"]
+         "-ffp-contract=fast",
+         # no v_pk_add/mul/fma_f32: hipcc makes them of ordinary float code, and some of their forms have given wrong results now and
+         # then.  (hipcc's host pass warns that it does not know the feature.)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():
