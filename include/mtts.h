@@ -20,7 +20,9 @@
 extern "C" {
 #endif
 
-enum { MTTS_ACT_NONE = 0, MTTS_ACT_RELU = 1, MTTS_ACT_TANH = 2, MTTS_ACT_SIGMOID = 3 };
+enum { MTTS_ACT_NONE = 0, MTTS_ACT_RELU = 1, MTTS_ACT_TANH = 2, MTTS_ACT_SIGMOID = 3,
+       MTTS_ACT_SILU = 4 /* z * sigmoid(z): group norm only */ };
+enum { MTTS_F32 = 0, MTTS_BF16 = 1 };      /* storage type of the tensors an argument block calls `dtype` */
 
 /* ---- general fp32 MFMA GEMM:  C[M,N] = epilogue(alpha * sum_k A(m,k) B(n,k)) ------------------------------
  * Replaces torch.nn.Linear / F.conv1d / their autograd GEMMs at: modules/tacotron2.py:34,111-112 (prenet,
@@ -125,6 +127,70 @@ typedef struct BnArgs {
 long mtts_bn_workspace_floats(int C);
 int mtts_bn_act_fwd(const BnArgs* args, void* stream);
 int mtts_bn_act_bwd(const BnArgs* args, void* stream);
+
+/* ---- group norm + activation + dropout, channel-last [N, L, C], fwd/bwd (csrc/group_norm.hip) ---------------------------------------
+ * The per-sample alternative to the BatchNorm of modules/layers.py:78-86.  Mean and variance of (sample, group) run over the sample's
+ * lengths[n] valid rows (clamped to [0, L]; NULL: all L) and the group's C / G channels; rows behind them are not read, y and dx are
+ * zero there.  Contiguous tensors of any alignment the type has; 16-byte addresses and C % 4 == 0 (bf16: % 8) take wide accesses. */
+typedef struct GroupNormArgs {
+    const void* x;         /* [N, L, C] of dtype; bwd: may be NULL where q holds it */
+    const float* gamma;    /* [C] */
+    const float* beta;     /* [C] */
+    const int* lengths;    /* [N] or NULL */
+    const uint8_t* mask;   /* [N, L, C] keep flags or NULL */
+    void* y;               /* fwd: [N, L, C] of dtype */
+    float* mean;           /* [N, G] written by fwd, read by bwd */
+    float* rstd;
+    int8_t* q;             /* [N, L, C] 8-bit checkpoint of x: written by fwd, read by bwd in place of x; NULL: none */
+    uint8_t* q_code;       /* [N, L, ceil(C / 32)] its exponents */
+    float* ws;             /* mtts_group_norm_workspace_floats(N, L, C, G) floats */
+    int N;
+    int L;
+    int C;
+    int G;
+    int dtype;             /* MTTS_F32 | MTTS_BF16: x, y, dy, dx */
+    int act;
+    float eps;
+    float mask_scale;
+    const void* dy;        /* bwd: [N, L, C] of dtype */
+    void* dx;
+    float* dgamma;         /* [C] or NULL */
+    float* dbeta;
+} GroupNormArgs;
+
+long mtts_group_norm_workspace_floats(int N, int L, int C, int G);
+int mtts_group_norm_act_fwd(const GroupNormArgs* args, void* stream);
+int mtts_group_norm_act_bwd(const GroupNormArgs* args, void* stream);
+
+/* ---- 8-bit activation checkpoints (csrc/checkpoint8.hip) ------------------------------------------------------------------------------
+ * q [N, L, C] signed bytes and code [N, L, ceil(C / 32)] biased exponents of x [N, L, C]: value = q * 2^(code - 127), one exponent per 32
+ * neighbouring channels of a row, the smallest that keeps |q| <= 127; |value - x| <= 2^(code - 128) (half a step; one step at magnitudes
+ * of 2^127 * 255/128 and more).  A block with an infinity or a NaN is NaN (code 255).  Rows behind lengths[n] (NULL: none) are zeros. */
+int mtts_checkpoint8_pack(const void* x, const int* lengths, int8_t* q, uint8_t* code, int N, int L, int C, int dtype, void* stream);
+int mtts_checkpoint8_unpack(const int8_t* q, const uint8_t* code, void* x, long rows, int C, int dtype, void* stream);
+
+/* ---- weight gradient of a 1-D convolution / linear layer from an 8-bit checkpoint of its input (csrc/wgrad8.hip) ----------------------
+ * dw[o, c, t] = sum_{n, l} dy[n, l, o] x[n, l + t * dilation - (kernel - 1) * dilation / 2, c], zero outside [0, L), groups as F.conv1d. */
+typedef struct Wgrad8Args {
+    const int8_t* q;       /* [N, L, I] */
+    const uint8_t* q_code; /* [N, L, ceil(I / 32)] */
+    const void* dy;        /* [N, L, O] of dtype */
+    float* dw;             /* [O, I / groups, kernel], or [O, kernel, I / groups] with packed != 0 */
+    float* ws;             /* mtts_conv_weight_grad8_workspace_floats floats (may be NULL where that is 0) */
+    int N;
+    int L;
+    int I;
+    int O;
+    int kernel;
+    int dilation;
+    int groups;
+    int dtype;             /* MTTS_F32 | MTTS_BF16: dy */
+    int packed;
+    int precision;         /* as GemmArgs.precision: 1 rounds an fp32 dy to bf16, 2 keeps all its bits, 0 the process-wide default */
+} Wgrad8Args;
+
+long mtts_conv_weight_grad8_workspace_floats(const Wgrad8Args* args);      /* -1: bad arguments (mtts_last_error) */
+int mtts_conv_weight_grad8(const Wgrad8Args* args, void* stream);
 
 /* ---- skinny GEMM (batch rows x streamed weight rows) with fused epilogues ----------------------------------
  * Replaces torch.nn.LSTMCell (modules/layers.py:18-47, called at modules/tacotron2.py:185,188), the attention

@@ -82,6 +82,8 @@ AdamArgs = STRUCTS["AdamArgs"]
 LstmPackArgs = STRUCTS["LstmPackArgs"]
 LstmStepArgs = STRUCTS["LstmStepArgs"]
 GenParamsArgs = STRUCTS["GenParamsArgs"]
+GroupNormArgs = STRUCTS["GroupNormArgs"]
+Wgrad8Args = STRUCTS["Wgrad8Args"]
 
 _lib = None
 
@@ -108,6 +110,8 @@ def lib():
         _lib.mtts_lstm_packed_weight_bytes.restype = ctypes.c_long
         _lib.mtts_gen_params_slabs.restype = ctypes.c_long
         _lib.mtts_gemm_planes_count.restype = ctypes.c_long
+        _lib.mtts_group_norm_workspace_floats.restype = ctypes.c_long
+        _lib.mtts_conv_weight_grad8_workspace_floats.restype = ctypes.c_long
         _lib.mtts_set_workspace.argtypes = [ctypes.c_void_p, ctypes.c_size_t]
         _lib.mtts_set_stream_workspace.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t]
     return _lib

@@ -14,7 +14,7 @@ int mtts_fail(const char* fmt, ...) {
 }
 
 MTTS_API const char* mtts_last_error(void) { return g_mtts_err; }
-MTTS_API int mtts_version(void) { return 102; }      // 102: DecoderGradArgs.part_ring (see mtts.h)
+MTTS_API int mtts_version(void) { return 103; }      // 102: DecoderGradArgs.part_ring; 103: group norm, 8-bit checkpoints (see mtts.h)
 
 // Bitmask of compile-time switches that make a build produce WRONG results by design (timing experiments).  The product sources have
 // none (round 4 removed the last two); the entry stays so that bindings keep refusing a library that reports anything but 0
@@ -39,6 +39,9 @@ MTTS_API int mtts_sizeof_struct(int which) {
         case 12: return (int)sizeof(LstmPackArgs);
         case 13: return (int)sizeof(LstmStepArgs);
         case 14: return (int)sizeof(GenParamsArgs);
+        // 15 stays the end mark of the structs above (bindings walk to the first -1)
+        case 16: return (int)sizeof(GroupNormArgs);
+        case 17: return (int)sizeof(Wgrad8Args);
         default: return -1;
     }
 }

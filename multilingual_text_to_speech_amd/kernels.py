@@ -81,33 +81,57 @@ def linear_bwd(x, weight, dy, need_dx=True):
     return dx, dW, db
 
 
+def _linear_bwd8(held, weight, dy, need_dx):
+    """linear_bwd with the input held as a Checkpoint8."""
+    N, K = weight.shape
+    dy2 = dy.reshape(-1, N)
+    dW = conv1d_weight_grad8(Checkpoint8(held.values.view(-1, K), held.scales.view(dy2.shape[0], -1)), dy2, 1).view(N, K)
+    db = colsum(dy2)
+    dx = None
+    if need_dx:
+        dx = _f32(dy2.shape[0], K, device=dy.device)
+        gemm(dy2, weight, dx, dy2.shape[0], K, N, N, K, K, transB=True)
+        dx = dx.view(held.values.shape)
+    return dx, dW, db
+
+
 class LinearFn(torch.autograd.Function):
-    """Linear (+ReLU +dropout) through the MFMA GEMM.  mask: uint8 keep flags or None."""
+    """Linear (+ReLU +dropout) through the MFMA GEMM.  mask: uint8 keep flags or None.  checkpoint: the input is saved in 8 bits (and
+    of the output only which values are positive)."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, act, mask, mask_scale):
+    def forward(ctx, x, weight, bias, act, mask, mask_scale, checkpoint=False):
         x = x.contiguous()
         y = linear_fwd(x, weight, bias, act, mask, mask_scale)
-        ctx.save_for_backward(x, weight, y, mask)
-        ctx.act, ctx.mask_scale, ctx.has_bias = act, mask_scale, bias is not None
+        if checkpoint:
+            held = checkpoint8(x)
+            ctx.save_for_backward(held.values, held.scales, weight, y > 0 if act == 1 else None, mask)
+        else:
+            ctx.save_for_backward(x, None, weight, y, mask)
+        ctx.act, ctx.mask_scale, ctx.has_bias, ctx.checkpoint = act, mask_scale, bias is not None, checkpoint
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, weight, y, mask = ctx.saved_tensors
+        x, scales, weight, y, mask = ctx.saved_tensors
         dz = dy.contiguous()
         if mask is not None:
             dz = dz * mask.view_as(dz) * ctx.mask_scale
         if ctx.act == 1:
-            dz = dz * (y > 0)
+            dz = dz * (y if ctx.checkpoint else y > 0)
         elif ctx.act != 0:
             raise NotImplementedError('LinearFn backward supports identity/relu')
-        dx, dW, db = linear_bwd(x, weight, dz, ctx.needs_input_grad[0])
-        return dx, dW, (db if ctx.has_bias else None), None, None, None
+        if ctx.checkpoint:
+            dx, dW, db = _linear_bwd8(Checkpoint8(x, scales), weight, dz, ctx.needs_input_grad[0])
+        else:
+            dx, dW, db = linear_bwd(x, weight, dz, ctx.needs_input_grad[0])
+        return dx, dW, (db if ctx.has_bias else None), None, None, None, None
 
 
-def linear(x, weight, bias=None, act='identity', mask=None, mask_scale=1.0):
-    return LinearFn.apply(x, weight, bias, ACT[act], mask, mask_scale)
+def linear(x, weight, bias=None, act='identity', mask=None, mask_scale=1.0, checkpoint=False):
+    """y = act(x W^T + b) [* dropout].  checkpoint=True saves x for the backward as a `Checkpoint8` (a quarter of its bytes): the weight
+    gradient is the one of the 8-bit values, everything else is unchanged."""
+    return LinearFn.apply(x, weight, bias, ACT[act], mask, mask_scale, checkpoint)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -295,13 +319,18 @@ def conv1d_bwd(x, wp, dy, k, dilation, groups, need_dx=True):
     # dW[o, t, c] = sum_r dy[r, o] * x[r + shift_t, c]   (one TN GEMM per tap through grid.z)
     gemm(dy, x, dwp, Og, Cg, R, O, Cin, k * Cg, transA=True, transB=True, seq_len=L, shift_mode=2, shift0=-p,
          dshift=dilation, batch=groups, zt=k, a_z=Og, b_z=Cg, c_z=Og * k * Cg, c_ztap=Cg)
-    dx = None
-    if need_dx:
-        dx = _f32(N_, L, Cin, device=x.device)
-        # dx[r, c] = sum_t sum_o dy[r - shift_t, o] * w[o, t, c]
-        gemm(dy, wp, dx, R, Cg, k * Og, O, k * Cg, Cin, transB=True, taps=k, Kc=Og, seq_len=L, shift_mode=1, shift0=p,
-             dshift=-dilation, b_tap=Cg, batch=groups, a_z=Og, b_z=Og * k * Cg, c_z=Cg)
-    return dx, dwp
+    return conv1d_input_grad(wp, dy, Cin, k, dilation, groups) if need_dx else None, dwp
+
+
+def conv1d_input_grad(wp, dy, Cin, k, dilation, groups):
+    """Input gradient of conv1d_fwd: dx [N, L, Cin]."""
+    N_, L, O = dy.shape
+    Cg, Og = Cin // groups, O // groups
+    dx = _f32(N_, L, Cin, device=dy.device)
+    # dx[r, c] = sum_t sum_o dy[r - shift_t, o] * w[o, t, c]
+    gemm(dy, wp, dx, N_ * L, Cg, k * Og, O, k * Cg, Cin, transB=True, taps=k, Kc=Og, seq_len=L, shift_mode=1, shift0=(k - 1) * dilation // 2,
+         dshift=-dilation, b_tap=Cg, batch=groups, a_z=Og, b_z=Og * k * Cg, c_z=Cg)
+    return dx
 
 
 def _bn_args(x2, gamma, beta, rmean, rvar, smean, srstd, mask, resid, y, ws, training, momentum, eps, act, mask_scale,
@@ -340,15 +369,23 @@ class ConvBnActFn(torch.autograd.Function):
         a = _bn_args(conv2, gamma.contiguous(), beta.contiguous(), rmean, rvar, smean, srstd, mask, x if highway else None, y, ws,
                      training, momentum, eps, act, mask_scale, groups if highway else 0)
         check(lib().mtts_bn_act_fwd(ctypes.byref(a), stream_ptr()), 'bn_act_fwd')
-        ctx.save_for_backward(x, wp, conv, gamma, beta, smean, srstd, mask)
+        ctx.checkpoint = len(cfg) > 10 and cfg[10]
+        held_x, held_conv = (checkpoint8(x), checkpoint8(conv)) if ctx.checkpoint else (None, None)
+        ctx.save_for_backward(held_x.values if held_x else x, wp, held_conv.values if held_conv else conv, gamma, beta, smean, srstd, mask,
+                              held_x.scales if held_x else None, held_conv.scales if held_conv else None)
         ctx.cfg, ctx.wshape = cfg, tuple(weight.shape)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, wp, conv, gamma, beta, smean, srstd, mask = ctx.saved_tensors
+        x, wp, conv, gamma, beta, smean, srstd, mask, x_scales, conv_scales = ctx.saved_tensors
         k, dilation, groups, act, training, momentum, eps, mask_scale, highway = ctx.cfg[:9]
         packed = len(ctx.cfg) > 9 and ctx.cfg[9]
+        held_x = None
+        if ctx.checkpoint:
+            held_x = Checkpoint8(x, x_scales)
+            conv = Checkpoint8(conv, conv_scales).unpack()
+            x = held_x.unpack() if highway else x
         N_, L, Cin = x.shape
         O = conv.shape[2]
         dev = x.device
@@ -361,17 +398,341 @@ class ConvBnActFn(torch.autograd.Function):
                      x if highway else None, None, ws, training, momentum, eps, act, mask_scale, groups if highway else 0)
         a.dy, a.dx, a.dgamma, a.dbeta, a.dresid = ptr(dy), ptr(dconv), ptr(dgamma), ptr(dbeta), ptr(dresid)
         check(lib().mtts_bn_act_bwd(ctypes.byref(a), stream_ptr()), 'bn_act_bwd')
-        dx, dwp = conv1d_bwd(x, wp, dconv, k, dilation, groups, ctx.needs_input_grad[0] or highway)
+        if ctx.checkpoint:
+            dx = conv1d_input_grad(wp, dconv, Cin, k, dilation, groups) if ctx.needs_input_grad[0] or highway else None
+            dw = conv1d_weight_grad8(held_x, dconv, k, dilation, groups, packed=packed)
+        else:
+            dx, dwp = conv1d_bwd(x, wp, dconv, k, dilation, groups, ctx.needs_input_grad[0] or highway)
+            dw = dwp if packed else unpack_conv_weight(dwp, *ctx.wshape)
         if highway:
             dx = dx + dresid
-        dw = dwp if packed else unpack_conv_weight(dwp, *ctx.wshape)
         return dx, dw, dgamma, dbeta, None, None, None, None
 
 
 def conv_bn_act(x, weight, gamma, beta, rmean, rvar, mask, *, kernel, dilation=1, groups=1, act='identity', training=True,
-                momentum=0.1, eps=1e-5, mask_scale=1.0, highway=False, packed=False):
-    cfg = (kernel, dilation, groups, ACT[act], training, momentum, eps, mask_scale, highway, packed)
+                momentum=0.1, eps=1e-5, mask_scale=1.0, highway=False, packed=False, checkpoint=False):
+    """checkpoint=True saves the block's input and the convolution's output for the backward as `Checkpoint8` (a quarter of their bytes)."""
+    cfg = (kernel, dilation, groups, ACT[act], training, momentum, eps, mask_scale, highway, packed, checkpoint)
     return ConvBnActFn.apply(x, weight, gamma, beta, rmean, rvar, mask, cfg)
+
+
+# ------------------------------------------------------------------------------------------------
+# 8-bit activation checkpoints, the weight gradient that reads them, group norm, channel-last
+# ------------------------------------------------------------------------------------------------
+
+CHECKPOINT_BLOCK = 32                      # neighbouring channels of a row that share an exponent
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1}
+GN_ACT = {**ACT, 'silu': 4}
+
+
+def _refuse(what, why):
+    raise _C.MttsError(f'{what}: {why}')
+
+
+def _check_storage(what, t, name):
+    if t.dtype not in _DTYPE:
+        _refuse(what, f'{name} is {t.dtype}: float32 or bfloat16 is expected')
+
+
+def _first_derivative_only(what):
+    if torch.is_grad_enabled():            # a backward under create_graph=True: its outputs would look like constants
+        _refuse(what, 'there is no second derivative (create_graph=True)')
+
+
+def _same_device(what, device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            _refuse(what, f'{name} is on {t.device}, the input on {device}')
+
+
+class _On:
+    """The launch's device is the tensors' own, whatever device is current."""
+    __slots__ = ('guard',)
+
+    def __init__(self, device):
+        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _check_lengths(what, lengths, N, L, device):
+    """Lengths [N], int32 or int64.  Host values are checked; values that already live on the device are clamped to [0, L] by the kernels."""
+    if lengths is None:
+        return None
+    if not isinstance(lengths, torch.Tensor):
+        lengths = torch.tensor(lengths, dtype=torch.int64)
+    if tuple(lengths.shape) != (N,) or lengths.dtype not in (torch.int32, torch.int64):
+        _refuse(what, f'lengths is {lengths.dtype} {tuple(lengths.shape)}: int32 or int64 of shape ({N},) is expected')
+    if lengths.is_cuda:
+        _same_device(what, device, lengths=lengths)
+    elif N and (int(lengths.min()) < 0 or int(lengths.max()) > L):
+        _refuse(what, f'lengths run from {int(lengths.min())} to {int(lengths.max())}: 0 to {L} is expected')
+    return lengths
+
+
+def _device_lengths(what, lengths, device):
+    if lengths is None:
+        return None
+    if not lengths.is_cuda and torch.cuda.is_current_stream_capturing():
+        _refuse(what, 'lengths have to be on the device while a graph is captured')
+    if lengths.is_cuda and lengths.dtype == torch.int64:
+        lengths = lengths.clamp(-1, 2 ** 31 - 1)              # the kernels' clamp to [0, L] must not see a wrapped value
+    return to_device_async(lengths, device, torch.int32).contiguous()
+
+
+class Checkpoint8:
+    """An activation in 8 bits: `values` int8 [..., C] and `scales` uint8 [..., ceil(C / 32)], biased exponents of one power of two per 32
+    neighbouring channels of a row.  It stands for values * 2^(scales - 127), which is exact in float32 and in bfloat16; a block with an
+    infinity or a NaN (exponent 255) stands for NaN.  `dtype` is the type that unpack() returns unless told otherwise."""
+    __slots__ = ('values', 'scales', 'dtype')
+
+    def __init__(self, values, scales, dtype=torch.float32):
+        if values.dtype != torch.int8 or scales.dtype != torch.uint8 or values.dim() < 1:
+            _refuse('Checkpoint8', f'values {values.dtype}, scales {scales.dtype}: int8 and uint8 are expected')
+        want = (*values.shape[:-1], -(-values.shape[-1] // CHECKPOINT_BLOCK))
+        if tuple(scales.shape) != want:
+            _refuse('Checkpoint8', f'scales have shape {tuple(scales.shape)}: {want} is expected for values of shape {tuple(values.shape)}')
+        if dtype not in _DTYPE:
+            _refuse('Checkpoint8', f'dtype is {dtype}: float32 or bfloat16 is expected')
+        _same_device('Checkpoint8', values.device, scales=scales)
+        self.values, self.scales, self.dtype = values.contiguous(), scales.contiguous(), dtype
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def nbytes(self):
+        return self.values.numel() + self.scales.numel()
+
+    def unpack(self, dtype=None):
+        """The values it stands for, [..., C]."""
+        dtype = dtype or self.dtype
+        if dtype not in _DTYPE:
+            _refuse('Checkpoint8.unpack', f'dtype is {dtype}: float32 or bfloat16 is expected')
+        require_gpu(self.values)
+        out = torch.empty(self.values.shape, dtype=dtype, device=self.values.device)
+        if out.numel():
+            C = out.shape[-1]
+            with _On(out.device):
+                check(lib().mtts_checkpoint8_unpack(ptr(self.values), ptr(self.scales), ptr(out), ctypes.c_long(out.numel() // C), C,
+                                                    _DTYPE[dtype], stream_ptr()), 'checkpoint8_unpack')
+        return out
+
+
+def checkpoint8(x, lengths=None):
+    """`Checkpoint8` of an activation [..., C] (float32 or bfloat16).  With `lengths` [N] for x [N, L, C] the rows behind a sample's length
+    are not read and stand for zeros.  The error is at most half of a step of the block's power of two (2^-7 of the block's largest
+    magnitude); magnitudes of 255/128 * 2^127 and more stop at 63/32 * 2^127."""
+    what = 'checkpoint8'
+    _check_storage(what, x, 'x')
+    if lengths is not None and x.dim() != 3:
+        _refuse(what, f'lengths need an input [N, L, C], not {tuple(x.shape)}')
+    if x.dim() < 1 or x.shape[-1] < 1:
+        _refuse(what, f'x has shape {tuple(x.shape)}: at least one channel is expected')
+    if lengths is not None:
+        lengths = _check_lengths(what, lengths, x.shape[0], x.shape[1], x.device)
+    require_gpu(x)
+    x = x.detach().contiguous()
+    C = x.shape[-1]
+    values = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], -(-C // CHECKPOINT_BLOCK)), dtype=torch.uint8, device=x.device)
+    if x.numel():
+        N, L = (x.shape[0], x.shape[1]) if lengths is not None else (1, x.numel() // C)
+        with _On(x.device):
+            lens = _device_lengths(what, lengths, x.device)
+            check(lib().mtts_checkpoint8_pack(ptr(x), ptr(lens), ptr(values), ptr(scales), N, L, C, _DTYPE[x.dtype], stream_ptr()), what)
+    return Checkpoint8(values, scales, x.dtype)
+
+
+def conv1d_weight_grad8(held, dy, kernel, dilation=1, groups=1, packed=False):
+    """Weight gradient of a 'same'-padded 1-D convolution from the `Checkpoint8` of its input [N, L, I] and dy [N, L, O] (float32 or
+    bfloat16): dW[o, c, t] = sum_{n, l} dy[n, l, o] x[n, l + t * dilation - (kernel - 1) * dilation // 2, c], float32 [O, I / groups, kernel]
+    (packed: [O, kernel, I / groups]).  kernel 1 takes inputs [..., I] of any shape: a linear layer.  A float32 dy keeps all its bits
+    unless set_precision('bf16') is on."""
+    what = 'conv1d_weight_grad8'
+    _check_storage(what, dy, 'dy')
+    if kernel < 1 or dilation < 1 or groups < 1:
+        _refuse(what, f'kernel {kernel}, dilation {dilation}, groups {groups}: whole numbers of 1 and more are expected')
+    if held.shape[:-1] != dy.shape[:-1] or dy.dim() < 1 or (kernel > 1 and dy.dim() != 3):
+        _refuse(what, f'input {tuple(held.shape)} and gradient {tuple(dy.shape)} do not belong to one convolution of kernel {kernel}')
+    _same_device(what, dy.device, checkpoint=held.values)
+    I, O = held.shape[-1], dy.shape[-1]
+    if I % groups or O % groups or not I or not O:
+        _refuse(what, f'{I} x {O} channels are not a multiple of {groups} groups')
+    require_gpu(held.values, dy)
+    shape = (O, kernel, I // groups) if packed else (O, I // groups, kernel)
+    rows = dy.numel() // O
+    if not rows:
+        return torch.zeros(shape, dtype=torch.float32, device=dy.device)
+    dy = dy.detach().contiguous()
+    dw = _f32(shape, device=dy.device)
+    N, L = (dy.shape[0], dy.shape[1]) if kernel > 1 else (1, rows)
+    a = _C.Wgrad8Args(held.values.data_ptr(), held.scales.data_ptr(), dy.data_ptr(), dw.data_ptr(), None, N, L, I, O, kernel, dilation, groups,
+                      _DTYPE[dy.dtype], int(packed), 0)
+    with _On(dy.device):
+        n = lib().mtts_conv_weight_grad8_workspace_floats(ctypes.byref(a))
+        if n < 0:
+            _refuse(what, lib().mtts_last_error().decode())
+        ws = _f32(n, device=dy.device) if n else None
+        a.ws = ptr(ws)
+        check(lib().mtts_conv_weight_grad8(ctypes.byref(a), stream_ptr()), what)
+    return dw
+
+
+def _gn_fwd(x, gamma, beta, groups, lengths, mask, act, eps, mask_scale, checkpoint):
+    """y, mean, rstd, checkpoint values / scales (or None) of contiguous operands."""
+    N, L, C = x.shape
+    dev = x.device
+    y = torch.empty_like(x)
+    stats = _f32(2, N, groups, device=dev)
+    q = torch.empty(x.shape, dtype=torch.int8, device=dev) if checkpoint else None
+    code = torch.empty(N, L, -(-C // CHECKPOINT_BLOCK), dtype=torch.uint8, device=dev) if checkpoint else None
+    if x.numel():
+        ws = _f32(lib().mtts_group_norm_workspace_floats(N, L, C, groups), device=dev)
+        a = _C.GroupNormArgs(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), ptr(lengths), ptr(mask), y.data_ptr(), stats.data_ptr(),
+                             stats.data_ptr() + 4 * N * groups, ptr(q), ptr(code), ws.data_ptr(), N, L, C, groups, _DTYPE[x.dtype], act, eps, mask_scale)
+        check(lib().mtts_group_norm_act_fwd(ctypes.byref(a), stream_ptr()), 'group_norm_act_fwd')
+    return y, stats, q, code
+
+
+def _gn_bwd(x, q, code, gamma, beta, stats, lengths, mask, dy, groups, act, eps, mask_scale):
+    """dx, dgamma, dbeta; x may be None where the checkpoint (q, code) holds it."""
+    N, L, C = dy.shape
+    dev = dy.device
+    dx = torch.empty_like(dy)
+    if not dy.numel():
+        return dx, torch.zeros_like(gamma), torch.zeros_like(beta)
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
+    ws = _f32(lib().mtts_group_norm_workspace_floats(N, L, C, groups), device=dev)
+    a = _C.GroupNormArgs(ptr(x), gamma.data_ptr(), beta.data_ptr(), ptr(lengths), ptr(mask), None, stats.data_ptr(),
+                         stats.data_ptr() + 4 * N * groups, ptr(q), ptr(code), ws.data_ptr(), N, L, C, groups, _DTYPE[dy.dtype], act, eps, mask_scale,
+                         dy.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr())
+    check(lib().mtts_group_norm_act_bwd(ctypes.byref(a), stream_ptr()), 'group_norm_act_bwd')
+    return dx, dgamma, dbeta
+
+
+class GroupNormActFn(torch.autograd.Function):
+    """Group norm + activation + dropout (mtts_group_norm_act_fwd / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, lengths, mask, cfg):
+        groups, act, eps, mask_scale, checkpoint = cfg
+        with _On(x.device):
+            y, stats, q, code = _gn_fwd(x, gamma, beta, groups, lengths, mask, act, eps, mask_scale, checkpoint)
+        ctx.save_for_backward(None if checkpoint else x, q, code, gamma, beta, stats, lengths, mask)
+        ctx.cfg = cfg
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        _first_derivative_only('group_norm_act')
+        x, q, code, gamma, beta, stats, lengths, mask = ctx.saved_tensors
+        groups, act, eps, mask_scale, _ = ctx.cfg
+        with _On(dy.device):
+            dx, dgamma, dbeta = _gn_bwd(x, q, code, gamma, beta, stats, lengths, mask, dy.contiguous(), groups, act, eps, mask_scale)
+        return dx, dgamma, dbeta, None, None, None
+
+
+def _gn_check(what, shape, device, gamma, beta, groups, lengths, mask, act):
+    """Contiguous gamma, beta, lengths (where they are) and uint8 flags, or a refusal."""
+    N, L, C = shape
+    if groups < 1 or C < 1 or C % groups:
+        _refuse(what, f'{C} channels are not a multiple of {groups} groups')
+    if act not in GN_ACT:
+        _refuse(what, f'unknown activation {act!r}: one of {", ".join(GN_ACT)} is expected')
+    for name, t in (('gamma', gamma), ('beta', beta)):
+        if t.dtype != torch.float32 or tuple(t.shape) != (C,):
+            _refuse(what, f'{name} is {t.dtype} {tuple(t.shape)}: float32 of shape ({C},) is expected')
+    if mask is not None:
+        if mask.dtype not in (torch.uint8, torch.bool) or tuple(mask.shape) != (N, L, C):
+            _refuse(what, f'mask is {mask.dtype} {tuple(mask.shape)}: uint8 keep flags of shape {(N, L, C)} are expected')
+        mask = mask.contiguous().view(torch.uint8)
+    _same_device(what, device, gamma=gamma, beta=beta, mask=mask)
+    return gamma.contiguous(), beta.contiguous(), _check_lengths(what, lengths, N, L, device), mask
+
+
+def group_norm_act(x, gamma, beta, groups, lengths=None, mask=None, *, act='identity', eps=1e-5, mask_scale=1.0, checkpoint=False):
+    """y = dropout(act(gamma * (x - mean) / sqrt(var + eps) + beta)) over x [N, L, C] channel-last, float32 or bfloat16 (gamma, beta:
+    float32).  Mean and (biased) variance of a sample's group run over its lengths[n] valid rows and the group's C / groups channels; rows
+    behind the length are never read, and y and the gradient of x are zero there.  act: identity, relu, tanh, sigmoid or silu;
+    mask: uint8 keep flags [N, L, C] with the factor mask_scale, as in conv_bn_act.
+    checkpoint=True saves x for the backward as a `Checkpoint8`: mean and deviation stay those of x, the gradients are those of the
+    8-bit values.  A backward that is captured into a graph has to be the only live graph of its leaves (torch's own rule: release the
+    eager one first)."""
+    what = 'group_norm_act'
+    _check_storage(what, x, 'x')
+    if x.dim() != 3:
+        _refuse(what, f'x has shape {tuple(x.shape)}: [N, L, C] is expected')
+    gamma, beta, lengths, mask = _gn_check(what, x.shape, x.device, gamma, beta, groups, lengths, mask, act)
+    require_gpu(x)
+    with _On(x.device):
+        lens, x = _device_lengths(what, lengths, x.device), x.contiguous()
+        if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
+            return GroupNormActFn.apply(x, gamma, beta, lens, mask, (groups, GN_ACT[act], eps, mask_scale, checkpoint))
+        return _gn_fwd(x, gamma, beta, groups, lens, mask, GN_ACT[act], eps, mask_scale, False)[0]
+
+
+class ConvGnActFn(torch.autograd.Function):
+    """pad -> conv1d(groups, dilation, no bias) -> group norm -> act -> dropout, channel-last: ConvBnActFn with statistics per sample."""
+
+    @staticmethod
+    def forward(ctx, x, weight, gamma, beta, lengths, mask, cfg):
+        k, dilation, groups, norm_groups, act, eps, mask_scale, checkpoint = cfg
+        with _On(x.device):
+            wp = pack_conv_weight(weight)
+            conv = conv1d_fwd(x, wp, k, dilation, groups)
+            y, stats, q, code = _gn_fwd(conv, gamma, beta, norm_groups, lengths, mask, act, eps, mask_scale, checkpoint)
+            held = checkpoint8(x) if checkpoint else None
+        if checkpoint:
+            ctx.save_for_backward(held.values, held.scales, None, q, code, wp, gamma, beta, stats, lengths, mask)
+        else:
+            ctx.save_for_backward(x, None, conv, None, None, wp, gamma, beta, stats, lengths, mask)
+        ctx.cfg, ctx.wshape = cfg, tuple(weight.shape)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        _first_derivative_only('conv_gn_act')
+        x, x_scales, conv, q, code, wp, gamma, beta, stats, lengths, mask = ctx.saved_tensors
+        k, dilation, groups, norm_groups, act, eps, mask_scale, checkpoint = ctx.cfg
+        with _On(dy.device):
+            dconv, dgamma, dbeta = _gn_bwd(conv, q, code, gamma, beta, stats, lengths, mask, dy.contiguous(), norm_groups, act, eps, mask_scale)
+            need_dx = ctx.needs_input_grad[0]
+            if checkpoint:
+                dx = conv1d_input_grad(wp, dconv, x.shape[2], k, dilation, groups) if need_dx else None
+                dw = conv1d_weight_grad8(Checkpoint8(x, x_scales), dconv, k, dilation, groups)
+            else:
+                dx, dwp = conv1d_bwd(x, wp, dconv, k, dilation, groups, need_dx)
+                dw = unpack_conv_weight(dwp, *ctx.wshape)
+        return dx, dw, dgamma, dbeta, None, None, None
+
+
+def conv_gn_act(x, weight, gamma, beta, lengths=None, mask=None, *, kernel, norm_groups, dilation=1, groups=1, act='identity', eps=1e-5,
+                mask_scale=1.0, checkpoint=False):
+    """The block of conv_bn_act with group norm over norm_groups groups in place of batch norm: x float32 [N, L, I], weight [O, I / groups,
+    kernel] -> [N, L, O].  The rows behind a sample's length take part in the convolution as they are (zeros, where the previous block was
+    this one) and are zeros in the output.  checkpoint=True saves the input and the convolution's output in 8 bits, and the weight
+    gradient is computed from the 8-bit input."""
+    what = 'conv_gn_act'
+    if x.dtype != torch.float32 or weight.dtype != torch.float32 or x.dim() != 3 or weight.dim() != 3:
+        _refuse(what, f'x {x.dtype} {tuple(x.shape)}, weight {weight.dtype} {tuple(weight.shape)}: float32 [N, L, I] and [O, I / groups, kernel] are expected')
+    if min(kernel, dilation, groups) < 1 or not x.numel() or tuple(weight.shape[1:]) != (x.shape[2] // groups, kernel) or x.shape[2] % groups or weight.shape[0] % groups:
+        _refuse(what, f'input {tuple(x.shape)} and weight {tuple(weight.shape)} do not belong to one convolution of kernel {kernel} with {groups} groups')
+    _same_device(what, x.device, weight=weight)
+    gamma, beta, lengths, mask = _gn_check(what, (x.shape[0], x.shape[1], weight.shape[0]), x.device, gamma, beta, norm_groups, lengths, mask, act)
+    require_gpu(x)
+    learns = torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, gamma, beta))
+    with _On(x.device):
+        lens = _device_lengths(what, lengths, x.device)
+        cfg = (kernel, dilation, groups, norm_groups, GN_ACT[act], eps, mask_scale, checkpoint and learns)
+        return ConvGnActFn.apply(x.contiguous(), weight, gamma, beta, lens, mask, cfg)
 
 
 class GenKernelFn(torch.autograd.Function):

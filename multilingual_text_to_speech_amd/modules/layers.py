@@ -9,7 +9,16 @@ from torch.nn import Sequential, Conv1d, BatchNorm1d, LSTMCell, Module
 
 from .. import kernels as K
 from ..masks import provider
+from ..params.params import Params as hp
 from .generated import Conv1dGenerated, BatchNorm1dGenerated
+
+
+def _checkpoint():
+    """hp.activation_checkpoint_bits = 8 (optional, not in the reference's parameters): the blocks save their activations in 8 bits."""
+    bits = getattr(hp, 'activation_checkpoint_bits', 32)
+    if bits not in (8, 32):
+        raise ValueError(f'activation_checkpoint_bits is {bits}: 8 or 32 is expected')
+    return bits == 8
 
 
 class _Slot(Module):
@@ -67,7 +76,8 @@ class ConvBlock(Module):
         return K.conv_bn_act(x, conv.weight, bn.weight, bn.bias, bn.running_mean, bn.running_var, mask,
                              kernel=self._kernel, dilation=self._dilation, groups=self._groups, act=self._activation_name,
                              training=training, momentum=bn.momentum, eps=bn.eps,
-                             mask_scale=1.0 / (1.0 - self._dropout_rate) if self._dropout_rate > 0 else 1.0, highway=highway)
+                             mask_scale=1.0 / (1.0 - self._dropout_rate) if self._dropout_rate > 0 else 1.0, highway=highway,
+                             checkpoint=training and _checkpoint())
 
     def forward(self, x, mask_name=None):
         return self._run(x, mask_name, False)
@@ -118,7 +128,7 @@ class ConvBlockGenerated(Module):
                              dilation=self._dilation, groups=self._groups, act=self._activation_name, training=training,
                              momentum=reg._momentum, eps=reg._eps,
                              mask_scale=1.0 / (1.0 - self._dropout_rate) if self._dropout_rate > 0 else 1.0, highway=highway,
-                             packed=packed)
+                             packed=packed, checkpoint=training and _checkpoint())
 
     def forward(self, e, x, mask_name=None):
         return self._run(e, x, mask_name, False)

@@ -1,0 +1,589 @@
+"""Group norm with an activation, 8-bit activation checkpoints and the weight gradient that reads them, on the GPU against their 64-bit
+definitions (tests/operator_refs.py, where the bounds are derived)."""
+import ctypes
+
+import pytest
+import torch
+
+from multilingual_text_to_speech_amd import _C
+from multilingual_text_to_speech_amd import kernels as K
+from tests import operator_refs as R
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def normal(gen, *shape, dtype=F32):
+    return torch.randn(*shape, generator=gen, device=DEV).to(dtype)
+
+
+def within(got, want, bound, what):
+    """|got - want| <= bound, elementwise, plus half a step of the result's own type."""
+    bound = bound + 1.01 * R.HALF[got.dtype] * (want.abs() + bound)
+    err = (got.double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()} values are off, the first by {err[bad][0].item():.3g} (bound {bound.expand_as(err)[bad][0].item():.3g})'
+
+
+def norm_case(seed, N, L, C, G, dtype, act, lengths=None, mask=False, offset=0.0, ckpt=False):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    x = (normal(gen, N, L, C) * torch.exp(0.3 * normal(gen, C)) + 0.5 * normal(gen, C) + offset).to(dtype)
+    gamma, beta = 1 + 0.2 * normal(gen, C), 0.2 * normal(gen, C)
+    keep = (torch.rand(N, L, C, generator=gen, device=DEV) < 0.6).to(torch.uint8) if mask else None
+    dy = normal(gen, N, L, C, dtype=dtype)
+    lens = None if lengths is None else torch.tensor(lengths, device=DEV)
+    if act == 'relu':            # its gradient jumps at z = 0: no gradient arrives where 64 and 32 bits could see different sides
+        z = R.group_norm(x, gamma, beta, G, lens, dy=dy, checkpoint=ckpt)['z_b']
+        dy = torch.where(z.abs() < 1e-2, torch.zeros_like(dy), dy)
+    return x, gamma, beta, keep, dy, lens
+
+
+def check_norm(x, gamma, beta, keep, dy, lens, G, act, ckpt, scale=1.0, eps=1e-5):
+    ref = R.group_norm(x, gamma, beta, G, lens, keep, act, eps, scale, dy=dy, checkpoint=ckpt)
+    ey, edx, edg, edb = R.norm_bounds(x, gamma, ref, dy, scale)
+    with torch.no_grad():
+        y0 = K.group_norm_act(x, gamma, beta, G, lens, keep, act=act, eps=eps, mask_scale=scale)
+    leaves = [t.detach().requires_grad_() for t in (x, gamma, beta)]            # not cloned: their alignment is part of the case
+    y = K.group_norm_act(*leaves, G, lens, keep, act=act, eps=eps, mask_scale=scale, checkpoint=ckpt)
+    assert torch.equal(y0, y)
+    dx, dgamma, dbeta = torch.autograd.grad(y, leaves, dy)
+    assert dx.dtype == x.dtype and dgamma.dtype == dbeta.dtype == F32
+    within(y.detach(), ref['y'], ey, 'y')
+    within(dx, ref['dx'], edx, 'dx')
+    within(dgamma, ref['dgamma'], edg, 'dgamma')
+    within(dbeta, ref['dbeta'], edb, 'dbeta')
+    behind = ~ref['valid'].expand_as(x)
+    assert not y[behind].any() and not dx[behind].any()
+    return y.detach(), dx
+
+
+# (N, L, C, G): one row, one value to a group's channel count, odd widths, vectors that straddle groups, one group, one channel per group,
+# the widths of the encoder and the post-net, long samples, more rows than a workgroup keeps
+SHAPES = [(1, 1, 512, 32), (1, 1, 8, 1), (3, 7, 80, 8), (2, 13, 37, 1), (2, 9, 35, 5), (2, 50, 6, 6), (4, 33, 12, 2), (5, 120, 512, 32),
+          (2, 600, 512, 16), (2, 257, 96, 3), (1, 1500, 64, 4), (1, 5000, 40, 2), (3, 431, 80, 8), (2, 65, 2560, 10), (1, 70, 4100, 2),
+          (2, 1025, 128, 4), (1, 2049, 256, 2), (70, 3, 64, 2), (2, 31, 1024, 1)]
+
+
+@pytest.mark.parametrize('ckpt', [False, True])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+def test_group_norm_shapes(shape, dtype, ckpt):
+    N, L, C, G = shape
+    x, gamma, beta, keep, dy, lens = norm_case(hash(shape) % 1000, N, L, C, G, dtype, 'tanh', ckpt=ckpt)
+    check_norm(x, gamma, beta, keep, dy, lens, G, 'tanh', ckpt)
+
+
+@pytest.mark.parametrize('ckpt', [False, True])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('act', list(R.ACTS))
+@pytest.mark.parametrize('shape', [(4, 45, 64, 4), (3, 29, 30, 5)], ids=str)
+def test_group_norm_activations_with_dropout_and_ragged_rows(shape, act, dtype, ckpt):
+    N, L, C, G = shape
+    lengths = [L, 0, 1, L - 3][:N]
+    x, gamma, beta, keep, dy, lens = norm_case(5, N, L, C, G, dtype, act, lengths, True, ckpt=ckpt)
+    check_norm(x, gamma, beta, keep, dy, lens, G, act, ckpt, scale=1 / 0.6)
+
+
+@pytest.mark.parametrize('L', [40, 700, 3000])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_rows_behind_the_length_are_never_read(L, dtype):
+    """NaN and infinities behind the lengths, and where dropout drops: the same bits as with zeros there."""
+    N, C, G = 4, 64, 2
+    lengths = [L, 0, L // 2, 1]
+    x, gamma, beta, keep, dy, lens = norm_case(9, N, L, C, G, dtype, 'silu', lengths, True)
+    behind = ~R.rows_valid(x, lens).expand_as(x)
+    outs = []
+    for fill, g in ((0.0, 0.0), (float('nan'), float('inf')), (torch.finfo(dtype).min, torch.finfo(dtype).min)):
+        xf = x.masked_fill(behind, fill).requires_grad_()
+        dyf = dy.masked_fill(behind, g).masked_fill(keep == 0, g)
+        for ckpt in (False, True):
+            y = K.group_norm_act(xf, gamma, beta, G, lens, keep, act='silu', mask_scale=2.0, checkpoint=ckpt)
+            outs.append((ckpt, y.detach(), *torch.autograd.grad(y, xf, dyf)))
+    for ckpt in (False, True):
+        same = [o[1:] for o in outs if o[0] == ckpt]
+        for o in same[1:]:
+            assert torch.equal(o[0], same[0][0]) and torch.equal(o[1], same[0][1])
+        assert torch.isfinite(same[0][0]).all() and torch.isfinite(same[0][1]).all()
+
+
+def test_a_non_finite_value_stays_in_its_group():
+    x, gamma, beta, _, dy, _ = norm_case(4, 3, 50, 64, 4, F32, 'tanh')
+    clean = K.group_norm_act(x, gamma, beta, 4)
+    x[1, 20, 17] = float('inf')
+    y = K.group_norm_act(x, gamma, beta, 4)
+    hit = torch.zeros_like(x, dtype=torch.bool)
+    hit[1, :, 16:32] = True
+    assert y[hit].isnan().all() and torch.equal(y[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize('offset', [100.0, 3000.0])
+@pytest.mark.parametrize('shape', [(2, 300, 64, 2), (1, 4000, 64, 2), (2, 33, 10, 2)], ids=str)
+def test_an_offset_costs_no_digits(shape, offset):
+    """Spread 1 around an offset: the second moment is centred, so the error stays in proportion to offset * 2^-24 (the bound's max|x|)."""
+    N, L, C, G = shape
+    x, gamma, beta, keep, dy, lens = norm_case(7, N, L, C, G, F32, 'tanh', offset=offset)
+    check_norm(x, gamma, beta, keep, dy, lens, G, 'tanh', False)
+
+
+def test_constant_groups_and_eps():
+    """Variance zero: xhat = 0, y = act(beta), dx = gamma dz minus its mean, over sqrt(eps)."""
+    x = torch.full((2, 20, 32), 5.0, device=DEV)
+    gamma, beta = torch.rand(32, device=DEV) + 0.5, torch.randn(32, device=DEV)
+    check_norm(x, gamma, beta, None, torch.randn_like(x), None, 2, 'sigmoid', False, eps=1e-3)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_strided_and_misaligned_operands(dtype):
+    """A transposed input, a sliced gradient, tensors that start one element behind an aligned address: the result of their copies."""
+    N, L, C, G = 3, 50, 64, 4
+    x, gamma, beta, _, dy, lens = norm_case(11, N, L, C, G, dtype, 'tanh', [50, 20, 0])
+    xt = x.transpose(1, 2).contiguous().transpose(1, 2)
+    store = torch.empty(x.numel() + 1, dtype=dtype, device=DEV)
+    xo = store[1:].view(N, L, C)
+    xo.copy_(x)
+    dys = torch.stack((dy, dy), 2)[:, :, 0]
+    g1 = torch.stack((gamma, gamma), 1)[:, 0]
+    results = []
+    for xx, dd, gg in ((x, dy, gamma), (xt, dys, g1)):
+        xx = xx.detach().requires_grad_()
+        y = K.group_norm_act(xx, gg, beta, G, lens, act='tanh')
+        results.append((y.detach(), *torch.autograd.grad(y, xx, dd)))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    check_norm(xo, gamma, beta, None, dy, lens, G, 'tanh', False)
+    check_norm(xo, gamma, beta, None, dy, lens, G, 'tanh', True)
+
+
+def test_differences_of_the_forward():
+    """<dx, v> against central differences of the kernel's own forward; the differences' truncation is taken from 64 bits, the rest is
+    the forward's rounding bound over 2h."""
+    x, gamma, beta, _, dy, _ = norm_case(13, 2, 9, 32, 4, F32, 'silu')
+    ref = R.group_norm(x, gamma, beta, 4, act='silu', dy=dy)
+    ey, edx, _, _ = R.norm_bounds(x, gamma, ref, dy)
+    v, h = torch.randn_like(x), 2.0 ** -6
+    xp, xm = x + h * v, x - h * v
+    f = lambda t: (K.group_norm_act(t, gamma, beta, 4, act='silu').double() * dy.double()).sum()  # noqa: E731
+    f64 = lambda t: (R.group_norm(t, gamma, beta, 4, act='silu')['y'] * dy.double()).sum()  # noqa: E731
+    xr = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(K.group_norm_act(xr, gamma, beta, 4, act='silu'), xr, dy)
+    slope = (dx.double() * v.double()).sum()
+    truncation = abs((f64(xp) - f64(xm)) / (2 * h) - (ref['dx'] * v.double()).sum())
+    rounding = 2 * (dy.double().abs().sum() * (ey + R.U * ref['y'].abs().max())) / (2 * h) + (edx + R.U) * v.double().abs().sum()
+    assert abs((f(xp) - f(xm)) / (2 * h) - slope) <= truncation + rounding
+
+
+def test_lengths_where_they_may_be():
+    x, gamma, beta, _, _, _ = norm_case(15, 3, 20, 32, 2, F32, 'tanh')
+    want = K.group_norm_act(x, gamma, beta, 2, torch.tensor([20, 3, 0], device=DEV, dtype=torch.int32))
+    for lengths in ([20, 3, 0], torch.tensor([20, 3, 0]), torch.tensor([20, 3, 0], device=DEV), torch.tensor([25, 3, -4], device=DEV),
+                    torch.tensor([2 ** 40, 3, -2 ** 40], device=DEV)):
+        assert torch.equal(K.group_norm_act(x, gamma, beta, 2, lengths), want)
+    assert K.group_norm_act(x[:0], gamma, beta, 2).shape == (0, 20, 32)
+    e = x[:, :0].clone().requires_grad_()
+    g = gamma.clone().requires_grad_()
+    y = K.group_norm_act(e, g, beta, 2)
+    assert y.shape == (3, 0, 32)
+    de, dg = torch.autograd.grad(y, (e, g), torch.zeros_like(y))
+    assert de.shape == e.shape and not dg.any()
+
+
+def test_no_second_derivative():
+    x = torch.randn(1, 4, 8, device=DEV, requires_grad=True)
+    y = K.group_norm_act(x, torch.ones(8, device=DEV), torch.zeros(8, device=DEV), 2)
+    with pytest.raises(_C.MttsError, match='second derivative'):
+        torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+
+
+# ---- checkpoints ----------------------------------------------------------------------------------------------------------------------
+
+def same_checkpoint(x, lengths=None):
+    held = K.checkpoint8(x, lengths)
+    q, code, values = R.round_trip(x, lengths)
+    assert torch.equal(held.values, q) and torch.equal(held.scales, code)
+    for dtype in (F32, BF16):
+        got = held.unpack(dtype)
+        assert got.dtype == dtype and torch.equal(got.double().nan_to_num(nan=12345.0), values.nan_to_num(nan=12345.0))
+    return held
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('shape', [(1, 1, 1), (1, 1, 32), (2, 3, 33), (5, 37, 80), (3, 11, 31), (2, 100, 512), (1, 1, 8200), (130, 1, 40), (7, 211, 1285)], ids=str)
+def test_checkpoint_equals_its_definition(shape, dtype):
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = (normal(gen, *shape) * torch.exp(3 * normal(gen, *shape[:2], 1))).to(dtype)
+    same_checkpoint(x)
+    N, L, _ = shape
+    lengths = torch.linspace(0, L, N, device=DEV).round().int()
+    xn = torch.where(R.rows_valid(x, lengths), x, torch.full_like(x, float('nan')))
+    held = same_checkpoint(xn, lengths)
+    assert not held.unpack()[~R.rows_valid(x, lengths).expand_as(x)].any()
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_checkpoint_of_every_kind_of_value(dtype):
+    """Ties, the quotient that would round to 128, subnormals, the topmost binade, zeros of both signs, non-finite blocks."""
+    big, tiny = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal
+    sub = tiny * 2.0 ** -5
+    rows = [[127.0, 0.5, 1.5, 2.5, -0.5, -1.5], [127.5, 1.0, 3.0], [127.25, -127.0, 63.5], [255.0, 1.0], [254.9, -3.0], [big, -big, 1.0, big / 64],
+            [big * 0.99, big / 128], [2.0 ** 127, 1.0], [tiny, -tiny / 2, sub], [sub, -sub], [0.0, -0.0], [float('inf'), 1.0], [float('-inf')],
+            [float('nan'), 2.0], [tiny * 127, tiny * 127.5], [1.9921875 * 2 ** 20, 2.0 ** 14, 2.0 ** 13, 3 * 2.0 ** 13]]
+    x = torch.zeros(len(rows), 96, device=DEV, dtype=dtype)
+    for i, r in enumerate(rows):
+        x[i, 32:32 + len(r)] = torch.tensor(r, device=DEV).to(dtype)
+    same_checkpoint(x)
+    same_checkpoint(x[:, :45].contiguous())
+
+
+def test_every_bfloat16_value_as_a_block_maximum():
+    x = torch.zeros(65536, 8, device=DEV, dtype=BF16)
+    x[:, 0] = torch.arange(-32768, 32768, device=DEV).to(torch.int16).view(BF16)
+    x[:, 5] = x[:, 0] / 3
+    same_checkpoint(x)
+
+
+def test_checkpoint_of_strided_misaligned_and_empty_inputs():
+    x = torch.randn(6, 7, 64, device=DEV)
+    want = K.checkpoint8(x)
+    t = K.checkpoint8(x.transpose(1, 2).contiguous().transpose(1, 2))
+    store = torch.empty(x.numel() + 1, device=DEV)
+    o = store[1:].view_as(x)
+    o.copy_(x)
+    for held in (t, K.checkpoint8(o)):
+        assert torch.equal(held.values, want.values) and torch.equal(held.scales, want.scales)
+    v = torch.empty(x.numel() + 1, dtype=torch.int8, device=DEV)[1:].view_as(x)
+    v.copy_(want.values)
+    assert torch.equal(K.Checkpoint8(v, want.scales).unpack(), want.unpack())
+    assert torch.equal(K.Checkpoint8(want.values[::2], want.scales[::2]).unpack(BF16), want.unpack(BF16)[::2])
+    empty = K.checkpoint8(x[:0])
+    assert empty.unpack().shape == (0, 7, 64) and empty.nbytes == 0
+
+
+# ---- weight gradient --------------------------------------------------------------------------------------------------------------------
+
+def grad_case(seed, N, L, I, O, dtype, code=None):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    held = K.checkpoint8(normal(gen, N, L, I) * torch.exp(normal(gen, N, L, 1)))
+    return held, normal(gen, N, L, O, dtype=dtype) * 1e-2
+
+
+def check_weight_grad(held, dy, k, d=1, g=1, rounded=False):
+    """Every product is exact or (a1 x, a2 x, a3 x) sums to it; one rounding of at most u of the magnitudes' sum for each product added, in
+    three terms of which two are small, and for each split: 1.02 R u + 64 u.  A gradient rounded to bf16 first adds 2^-8 of the magnitudes."""
+    want, size = R.weight_grad(held.unpack().double(), dy, k, d, g)
+    rows = dy.numel() // dy.shape[-1]
+    bound = ((1.02 * rows + 64) * R.U + (2.0 ** -8 if rounded else 0)) * size
+    got = K.conv1d_weight_grad8(held, dy, k, dilation=d, groups=g)
+    assert got.dtype == F32 and got.shape == want.shape
+    within(got, want, bound, 'dW')
+    packed = K.conv1d_weight_grad8(held, dy, k, dilation=d, groups=g, packed=True)
+    assert torch.equal(packed.permute(0, 2, 1), got)
+    return got
+
+
+# (N, L, I, O, kernel, dilation, groups): one row, samples shorter than the kernel, widths that are no multiple of four, of a block or of a
+# tile, groups that start inside a block, many rows (split), wide outputs
+GRADS = [(1, 1, 4, 4, 1, 1, 1), (1, 1, 64, 32, 5, 1, 1), (3, 2, 32, 64, 5, 1, 1), (2, 9, 80, 512, 5, 1, 1), (7, 211, 80, 96, 5, 1, 1), (4, 31, 37, 21, 3, 2, 1),
+         (3, 50, 60, 36, 3, 9, 3), (2, 40, 70, 30, 7, 3, 5), (5, 133, 640, 320, 3, 9, 5), (16, 120, 512, 512, 5, 1, 1), (2, 700, 256, 130, 1, 1, 1),
+         (64, 600, 32, 64, 3, 1, 1), (1, 5000, 100, 100, 2, 1, 1), (3, 17, 48, 48, 4, 3, 1), (2, 12, 64, 64, 31, 5, 1), (2, 100, 1040, 260, 1, 1, 2)]
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('case', GRADS, ids=str)
+def test_weight_grad_shapes(case, dtype):
+    N, L, I, O, k, d, g = case
+    held, dy = grad_case(sum(case), N, L, I, O, dtype)
+    check_weight_grad(held, dy, k, d, g)
+
+
+def test_weight_grad_keeps_every_bit_of_a_float32_gradient():
+    """One product per output: the three terms add up to the rounded product of the float32 gradient."""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.zeros(1, 64, device=DEV)
+    x[0] = torch.randint(1, 127, (64,), generator=gen, device=DEV).float()
+    x[0, ::32] = 127.0
+    dy = normal(gen, 1, 96) * torch.exp(8 * normal(gen, 1, 96))
+    got = K.conv1d_weight_grad8(K.checkpoint8(x), dy, 1)[:, :, 0]
+    want = dy.double().t() * x.double()
+    assert ((got.double() - want).abs() <= 2.001 * R.U * want.abs()).all()          # three terms: two additions
+
+
+def test_weight_grad_in_bf16_mode_rounds_the_gradient():
+    held, dy = grad_case(21, 4, 60, 64, 64, F32)
+    try:
+        _C.set_precision('bf16')
+        got = check_weight_grad(held, dy, 3, rounded=True)
+        again = K.conv1d_weight_grad8(held, dy.bfloat16(), 3)
+    finally:
+        _C.set_precision('fp32')
+    assert torch.equal(got, again)
+
+
+def test_weight_grad_of_strided_and_misaligned_operands():
+    held, dy = grad_case(23, 3, 40, 64, 48, F32)
+    want = check_weight_grad(held, dy, 3)
+    store = torch.empty(dy.numel() + 1, device=DEV)
+    o = store[1:].view_as(dy)
+    o.copy_(dy)
+    v = torch.empty(held.values.numel() + 1, dtype=torch.int8, device=DEV)[1:].view_as(held.values)
+    v.copy_(held.values)
+    assert torch.equal(K.conv1d_weight_grad8(held, dy.transpose(0, 1).contiguous().transpose(0, 1), 3), want)
+    check_weight_grad(K.Checkpoint8(v, held.scales), o, 3)
+
+
+def test_weight_grad_of_no_rows_and_of_a_lost_block():
+    held, dy = grad_case(25, 2, 8, 64, 16, F32)
+    none = K.conv1d_weight_grad8(K.Checkpoint8(held.values[:0], held.scales[:0]), dy[:0], 3)
+    assert none.shape == (16, 64, 3) and not none.any()
+    scales = held.scales.clone()
+    scales[1, 4, 1] = 255
+    values = held.values.clone()
+    values[1, 4, 32:] = 0
+    got = K.conv1d_weight_grad8(K.Checkpoint8(values, scales), dy, 3)
+    assert got[:, 32:].isnan().all() and torch.isfinite(got[:, :32]).all()
+
+
+def test_repeated_calls_return_the_same_bits():
+    """Sums have a fixed order: nothing depends on which workgroup ends first."""
+    held, dy = grad_case(27, 16, 300, 128, 128, F32)
+    x, gamma, beta, keep, g, lens = norm_case(27, 8, 700, 128, 4, F32, 'tanh')
+    first = None
+    for _ in range(3):
+        xr, gr, br = (t.detach().clone().requires_grad_() for t in (x, gamma, beta))
+        y = K.group_norm_act(xr, gr, br, 4, act='tanh', checkpoint=True)
+        now = (K.conv1d_weight_grad8(held, dy, 5), y.detach(), *torch.autograd.grad(y, (xr, gr, br), g))
+        assert first is None or all(torch.equal(a, b) for a, b in zip(now, first))
+        first = now
+
+
+# ---- together -----------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('ckpt', [False, True])
+@pytest.mark.parametrize('groups,d', [(1, 1), (2, 3)])
+def test_conv_block_against_its_definition(groups, d, ckpt):
+    """conv -> group norm -> tanh -> dropout and its gradients, each stage in 64 bits from the kernel's own convolution output (a value
+    next to a border of the 8-bit rounding would fall to the other side otherwise).  The convolutions are fp32-accurate products: their
+    error is below rows u of the magnitudes."""
+    N, L, I, O, k, G = 4, 60, 64, 96, 5, 6
+    gen = torch.Generator(device=DEV).manual_seed(31)
+    x, w = normal(gen, N, L, I), normal(gen, O, I // groups, k) / (I // groups * k) ** 0.5
+    gamma, beta, dy = 1 + 0.1 * normal(gen, O), 0.1 * normal(gen, O), normal(gen, N, L, O)
+    keep = (torch.rand(N, L, O, generator=gen, device=DEV) < 0.5).to(torch.uint8)
+    lens = torch.tensor([60, 41, 0, 7], device=DEV)
+    x = x * R.rows_valid(x, lens)
+    leaves = [t.clone().requires_grad_() for t in (x, w, gamma, beta)]
+    y = K.conv_gn_act(*leaves, lens, keep, kernel=k, norm_groups=G, dilation=d, groups=groups, act='tanh', mask_scale=2.0, checkpoint=ckpt)
+    dx, dw, dgamma, dbeta = torch.autograd.grad(y, leaves, dy)
+    c = K.conv1d_fwd(x, K.pack_conv_weight(w), k, d, groups)
+    want_c = R.conv(x.double(), w.double(), d, groups)
+    within(c, want_c, 2 * I * k * R.U * R.conv(x.double().abs(), w.double().abs(), d, groups), 'conv')
+    ref = R.group_norm(c, gamma, beta, G, lens, keep, 'tanh', 1e-5, 2.0, dy=dy, checkpoint=ckpt)
+    ey, edc, edg, edb = R.norm_bounds(c, gamma, ref, dy, 2.0)
+    within(y.detach(), ref['y'], ey, 'y')
+    within(dgamma, ref['dgamma'], edg, 'dgamma')
+    within(dbeta, ref['dbeta'], edb, 'dbeta')
+    dc = ref['dx']
+    held = R.round_trip(x)[2] if ckpt else x.double()
+    want, size = R.weight_grad(held, dc, k, d, groups)
+    _, ones = R.weight_grad(held, torch.ones_like(dc), k, d, groups)
+    within(dw, want, 4 * N * L * R.U * size + (edc + R.U * dc.abs().max()) * ones, 'dW')
+    wt = w.double().reshape(groups, O // groups, I // groups, k).transpose(1, 2).flip(-1).reshape(I, O // groups, k)
+    full = lambda a, b: R.conv(a, b, d, groups)  # noqa: E731  (k odd: the transposed convolution is a 'same' convolution too)
+    within(dx, full(dc, wt), 4 * O * k * R.U * full(dc.abs(), wt.abs()) + (edc + R.U * dc.abs().max()) * full(torch.ones_like(dc), wt.abs()), 'dx')
+
+
+def _saved_bytes(f):
+    total = [0]
+
+    def pack(t):
+        total[0] += t.numel() * t.element_size()
+        return t
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        out = f()
+    return out, total[0]
+
+
+def test_two_blocks_and_a_linear_layer_train_from_checkpoints():
+    """A run as it would be used: two blocks and a projection; the checkpointed gradients stay within the rounding of the 8-bit values
+    (half a step is 2^-7 of a block's largest value, about 1.4 % of the values' own size on average, over two blocks) and the saved bytes
+    fall to less than a half (the weights and flags among them)."""
+    N, L, I, H, M = 8, 120, 80, 128, 84
+    gen = torch.Generator(device=DEV).manual_seed(37)
+    p = [normal(gen, H, I, 5) / 20, 1 + 0.1 * normal(gen, H), 0.1 * normal(gen, H), normal(gen, H, H, 5) / 25, 1 + 0.1 * normal(gen, H),
+         0.1 * normal(gen, H), normal(gen, M, H) / 11, normal(gen, M)]
+    x, dy = normal(gen, N, L, I), normal(gen, N, L, M)
+    lens = torch.linspace(10, L, N, device=DEV).int()
+    got = {}
+    for ckpt in (False, True):
+        leaves = [t.clone().requires_grad_() for t in p]
+
+        def net():
+            h = K.conv_gn_act(x, leaves[0], leaves[1], leaves[2], lens, kernel=5, norm_groups=4, act='tanh', checkpoint=ckpt)
+            h = K.conv_gn_act(h, leaves[3], leaves[4], leaves[5], lens, kernel=5, norm_groups=4, act='silu', checkpoint=ckpt)
+            return K.linear(h, leaves[6], leaves[7], checkpoint=ckpt)
+        y, saved = _saved_bytes(net)
+        got[ckpt] = (y.detach(), torch.autograd.grad(y, leaves, dy), saved)
+    assert torch.equal(got[False][0], got[True][0])                  # the forward does not change
+    assert got[True][2] < 0.5 * got[False][2]
+    for a, b in zip(got[True][1], got[False][1]):
+        rel = ((a - b).norm() / b.norm()).item()
+        assert rel < 0.06, rel
+    assert torch.equal(got[True][1][7], got[False][1][7])            # the bias sees no checkpoint
+
+
+@pytest.mark.parametrize('act', ['identity', 'relu'])
+def test_linear_from_a_checkpoint(act):
+    gen = torch.Generator(device=DEV).manual_seed(41)
+    x, w, b, dy = normal(gen, 5, 33, 80), normal(gen, 36, 80), normal(gen, 36), normal(gen, 5, 33, 36)
+    keep = (torch.rand(5, 33, 36, generator=gen, device=DEV) < 0.5).to(torch.uint8)
+    out = {}
+    for ckpt in (False, True):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        y = K.linear(*leaves, act, keep, 2.0, checkpoint=ckpt)
+        out[ckpt] = (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    for i in (0, 1, 3):
+        assert torch.equal(out[True][i], out[False][i])
+    dz = dy.double() * keep * 2 * ((out[True][0] > 0) if act == 'relu' else 1)
+    held = R.round_trip(x)[2]
+    want, size = R.weight_grad(held.reshape(1, -1, 80), dz.reshape(1, -1, 36), 1)
+    within(out[True][2], want[:, :, 0], (1.02 * 165 + 64) * R.U * size[:, :, 0], 'dW')
+
+
+@pytest.mark.parametrize('highway,groups', [(False, 1), (True, 2)])
+def test_batch_norm_block_from_checkpoints(highway, groups):
+    """conv_bn_act: same forward bits; dW from the 8-bit input, the rest from the 8-bit convolution output."""
+    gen = torch.Generator(device=DEV).manual_seed(43)
+    N, L, I = 6, 50, 64
+    O = 2 * I if highway else 96
+    x, w = normal(gen, N, L, I), normal(gen, O, I // groups, 3) / 14
+    gamma, beta, dy = 1 + 0.1 * normal(gen, O), 0.1 * normal(gen, O), normal(gen, N, L, I if highway else O)
+    out = {}
+    for ckpt in (False, True):
+        leaves = [t.clone().requires_grad_() for t in (x, w, gamma, beta)]
+        rm, rv = torch.zeros(O, device=DEV), torch.ones(O, device=DEV)
+        y, saved = _saved_bytes(lambda: K.conv_bn_act(*leaves, rm, rv, None, kernel=3, groups=groups, act='tanh', highway=highway, checkpoint=ckpt))
+        out[ckpt] = (y.detach(), rm, rv, torch.autograd.grad(y, leaves, dy), saved)
+    assert all(torch.equal(a, b) for a, b in zip(out[False][:3], out[True][:3]))
+    assert out[True][4] < 0.6 * out[False][4]
+    for a, b in zip(out[True][3], out[False][3]):
+        rel = ((a - b).norm() / b.norm()).item()
+        assert 0 < rel < 0.06, rel
+
+
+def test_model_block_takes_the_option(monkeypatch):
+    from multilingual_text_to_speech_amd.modules.layers import ConvBlock
+    from multilingual_text_to_speech_amd.params.params import Params as hp
+    block = ConvBlock(64, 128, 5, 0.0, 'tanh').to(DEV)
+    x = torch.randn(4, 40, 64, device=DEV)
+    y0, full = _saved_bytes(lambda: block(x, 'b'))
+    monkeypatch.setattr(hp, 'activation_checkpoint_bits', 8, raising=False)
+    y1, held = _saved_bytes(lambda: block(x, 'b'))
+    # 160 rows of input and convolution output: 4 bytes a value become 1 and a byte per 32 channels; weights and statistics stay
+    assert torch.equal(y0, y1) and full - held == 4 * 160 * (64 + 128) - 160 * (64 + 2 + 128 + 4)
+    block.eval()
+    assert torch.isfinite(block(x, 'b')).all()
+
+
+# ---- streams, graphs, sizes ---------------------------------------------------------------------------------------------------------------
+
+def test_two_streams_at_once():
+    """Workspaces are the call's own: two streams run the operators at once and return what each returns alone."""
+    cases = [norm_case(s, 8, 300, 128, 4, F32, 'tanh') for s in (51, 52)]
+    grads = [grad_case(s, 16, 300, 128, 128, F32) for s in (53, 54)]
+
+    def work(i):
+        x, gamma, beta, _, dy, _ = cases[i]
+        xr = x.detach().requires_grad_()
+        y = K.group_norm_act(xr, gamma, beta, 4, act='tanh', checkpoint=True)
+        return [y.detach(), *torch.autograd.grad(y, xr, dy), K.conv1d_weight_grad8(*grads[i], 5)]
+    alone = [work(0), work(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(work(i))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(a, b) for r in got[i] for a, b in zip(r, alone[i]))
+
+
+def test_captured_and_replayed():
+    """Forward, checkpoint, weight gradient and backward in two graphs that share nothing, replayed with eager work between."""
+    x, gamma, beta, _, dy, lens = norm_case(61, 6, 200, 64, 4, F32, 'silu', [200, 150, 0, 33, 1, 199])
+    held0, g0 = grad_case(62, 6, 200, 64, 96, F32)
+    lens = lens.int()
+
+    def step(xs, ds):
+        y = K.group_norm_act(xs, gamma, beta, 4, lens, act='silu', checkpoint=True)
+        dx, = torch.autograd.grad(y, xs, ds)
+        return y.detach(), dx, K.conv1d_weight_grad8(K.checkpoint8(xs, lens), g0, 3), K.checkpoint8(dx).unpack()
+    inputs = [(x.clone().requires_grad_(), dy.clone()) for _ in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for a in inputs:
+            step(*a)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for a in inputs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(*a))
+        graphs.append(g)
+    gen = torch.Generator(device=DEV).manual_seed(63)
+    for r in range(4):
+        for i in (0, 1):
+            with torch.no_grad():
+                inputs[i][0].copy_(normal(gen, *x.shape))
+                inputs[i][1].copy_(normal(gen, *x.shape))
+        graphs[r % 2].replay()
+        graphs[1 - r % 2].replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            want = step(inputs[i][0].detach().clone().requires_grad_(), inputs[i][1])
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], want))
+
+
+def test_host_lengths_are_refused_during_capture():
+    x = torch.randn(2, 8, 32, device=DEV)
+    w = torch.ones(32, device=DEV)
+    K.group_norm_act(x, w, w, 2)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(_C.MttsError, match='captured'):
+            K.group_norm_act(x, w, w, 2, [8, 3])
+
+
+@pytest.mark.parametrize('dtype', [BF16])
+def test_more_than_2_to_the_31_values(dtype):
+    """The last of three samples starts behind 2^31 values: the same bits as alone."""
+    L, C, G = 262200, 4096, 32
+    x = torch.empty(3, L, C, dtype=dtype, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(71)
+    piece = normal(gen, 1024, C, dtype=dtype)
+    for n in range(3):
+        x[n] = piece.repeat(-(-L // 1024), 1)[:L] * (n + 1)
+    w, b = torch.ones(C, device=DEV), torch.zeros(C, device=DEV)
+    lens = torch.tensor([1, 1, 500], device=DEV)
+    y = K.group_norm_act(x, w, b, G, lens, act='tanh')
+    ref = R.group_norm(x[2:, :500], w, b, G, act='tanh')
+    within(y[2:, :500], ref['y'], R.norm_bounds(x[2:, :500], w, ref), 'y')
+    assert not y[2, 500:].any() and not y[0, 1:].any()
+    del y
+    held = K.checkpoint8(x, lens)
+    tail = K.checkpoint8(x[2, :500])
+    assert torch.equal(held.values[2, :500], tail.values) and torch.equal(held.scales[2, :500], tail.scales)
+    assert torch.equal(held.unpack()[2, :500], tail.unpack())
+    # the backward's last rows
+    xr = x[:, :, :].requires_grad_()
+    full = torch.tensor([1, 1, L], device=DEV)
+    dx, = torch.autograd.grad(K.group_norm_act(xr, w, b, G, full, checkpoint=True), xr, x.detach())
+    assert torch.isfinite(dx[2, -64:]).all() and dx[2, -64:].float().abs().max() > 0
+
+
+def test_entry_point_error_text_reaches_python():
+    held, dy = grad_case(81, 1, 4, 32, 32, F32)
+    a = _C.Wgrad8Args(held.values.data_ptr(), held.scales.data_ptr(), dy.data_ptr(), None, None, 1, 4, 32, 32, 3, 1, 1, 0, 0, 0)
+    with pytest.raises(_C.MttsError, match='missing tensor'):
+        _C.check(_C.lib().mtts_conv_weight_grad8(ctypes.byref(a), _C.stream_ptr()), 'conv1d_weight_grad8')
