@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(CK_T) ck_pack_kernel(const T* __restrict__ x, 
 #pragma unroll
         for (int u = 0; u < CK_U; ++u) {
             float f[VEC];
-            v[u].get(f);
+            get_vec(v[u], f);
             unsigned m = 0;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) m = umax_(m, abs_bits(f[j]));

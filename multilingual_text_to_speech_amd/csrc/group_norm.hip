@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(GN_T) gn_moments_kernel(GroupNormArgs p, int c
             const float inv = 1.f / (float)k;
             float f[GN_U][VEC];
 #pragma unroll
-            for (int u = 0; u < GN_U; ++u) v[u].get(f[u]);
+            for (int u = 0; u < GN_U; ++u) get_vec(v[u], f[u]);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 float s = 0.f, q = 0.f;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(GN_T) gn_apply_kernel(GroupNormArgs p, int chu
             const int rr = r + u * t.TY;
             if (rr >= t.r1) break;
             float f[VEC];
-            v[u].get(f);
+            get_vec(v[u], f);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) f[j] = (f[j] - k.mean[j]) * k.rstd[j] * k.gamma[j] + k.beta[j];
             gn_act<VEC>(p.act, f);
@@ -237,12 +237,12 @@ template <typename T, int VEC, bool CK> struct GnBwdRow {
     }
     __device__ __forceinline__ void get(const GroupNormArgs& p, const GnCol<VEC>& k, float (&xhat)[VEC], float (&dz)[VEC]) const {
         float z[VEC];
-        dy.get(dz);
+        get_vec(dy, dz);
         if (CK) {
             const float s = ck_scale(code);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) xhat[j] = ck_value(q.get(j), s);
-        } else x.get(xhat);
+        } else get_vec(x, xhat);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             xhat[j] = (xhat[j] - k.mean[j]) * k.rstd[j];

@@ -15,9 +15,7 @@ __device__ __forceinline__ float bf16_hi(unsigned w) { return __uint_as_float(w 
 // two fp32 -> two bf16 in one word, round to nearest even (v_cvt_pk_bf16_f32): off by half a step at most, 2^-8 of the value
 __device__ __forceinline__ unsigned bf16_pack(float a, float b) {
     const f32x2_t f = {a, b};
-    const bf16x2_t h = __builtin_convertvector(f, bf16x2_t);
-    unsigned w; __builtin_memcpy(&w, &h, 4);
-    return w;
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f, bf16x2_t));
 }
 
 // VEC values as they lie in memory: one 16-byte access (4 fp32 / 8 bf16), or one element (VEC = 1) where the width or an address does
@@ -26,33 +24,38 @@ template <typename T, int VEC> struct Raw;
 template <> struct Raw<float, 4> {
     u32x4 w;
     __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const u32x4*>(p); }
-    __device__ __forceinline__ void get(float* f) const {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(w[j]);
-    }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned at) { w = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0); }
+    __device__ __forceinline__ float at(int j) const { return __uint_as_float(w[j]); }
     __device__ __forceinline__ void zero() { w = u32x4{0, 0, 0, 0}; }
+};
+template <> struct Raw<bf16_t, 4> {
+    u32x2 w;
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned at) { w = __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0); }
+    __device__ __forceinline__ float at(int j) const { return j & 1 ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]); }
 };
 template <> struct Raw<bf16_t, 8> {
     u32x4 w;
     __device__ __forceinline__ void load(const bf16_t* p) { w = *reinterpret_cast<const u32x4*>(p); }
-    __device__ __forceinline__ void get(float* f) const {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { f[2 * j] = bf16_lo(w[j]); f[2 * j + 1] = bf16_hi(w[j]); }
-    }
+    __device__ __forceinline__ float at(int j) const { return j & 1 ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]); }
     __device__ __forceinline__ void zero() { w = u32x4{0, 0, 0, 0}; }
 };
 template <> struct Raw<float, 1> {
     float w;
     __device__ __forceinline__ void load(const float* p) { w = *p; }
-    __device__ __forceinline__ void get(float* f) const { f[0] = w; }
+    __device__ __forceinline__ float at(int) const { return w; }
     __device__ __forceinline__ void zero() { w = 0.f; }
 };
 template <> struct Raw<bf16_t, 1> {
     uint16_t w;
     __device__ __forceinline__ void load(const bf16_t* p) { w = p->v; }
-    __device__ __forceinline__ void get(float* f) const { f[0] = __uint_as_float((unsigned)w << 16); }
+    __device__ __forceinline__ float at(int) const { return __uint_as_float((unsigned)w << 16); }
     __device__ __forceinline__ void zero() { w = 0; }
 };
+
+template <typename T, int VEC> __device__ __forceinline__ void get_vec(const Raw<T, VEC>& r, float (&f)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = r.at(j);
+}
 
 __device__ __forceinline__ void store_vec(float* p, const float (&f)[4]) { *reinterpret_cast<f32x4*>(p) = f32x4{f[0], f[1], f[2], f[3]}; }
 __device__ __forceinline__ void store_vec(float* p, const float (&f)[1]) { *p = f[0]; }

@@ -25,155 +25,225 @@ __device__ __forceinline__ unsigned top_halves(float lo, float hi) {      // the
 }
 __device__ __forceinline__ float bf16_head(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
-// TERMS 3: exact split of fp32; 1: bf16 gradient, or fp32 rounded.  VEC: quads of columns are loaded at once (else element by element).
-template <typename T, int TERMS, int TM, int TN, int WM, int WN, bool VEC>
-__global__ void __launch_bounds__((TM / WM) * (TN / WN) * 64) wgrad8_kernel(Wgrad8Args p, int splits, int tiles_n, int steps_per) {
-    constexpr int THREADS = (TM / WM) * (TN / WN) * 64, FM = WM / 32, FN = WN / 32;
-    static_assert(TM + TN <= THREADS, "one 8 x 4 piece of an operand tile per thread");
-    __shared__ u32x4 sa[TERMS][TM * 4];
-    __shared__ u32x4 sb[TN * 4];
-    const int Og = p.O / p.groups, Cg = p.I / p.groups, Nn = p.kernel * Cg, nb = (p.I + CK_BLOCK - 1) / CK_BLOCK;
-    const int split = blockIdx.z % splits, g = blockIdx.z / splits;
-    const int tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n;
-    const int m0 = tm * TM, n0 = tn * TN;
-    const long R = (long)p.N * p.L;
-    const long k_begin = (long)split * steps_per * WG_BK, k_end = min(R, k_begin + (long)steps_per * WG_BK);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = (wave / (TN / WN)) * WM, wn = (wave % (TN / WN)) * WN;
-
-    // this thread's piece: threads [0, TM) stage dy, [TM, TM + TN) stage x; 4 columns, row octet `oct` of the step
-    const bool is_a = tid < TM, is_b = !is_a && tid < TM + TN;
-    const int piece = is_a ? tid : tid - TM, quads = (is_a ? TM : TN) / 4;
-    const int oct = piece / quads, col = (piece - oct * quads) * 4;
-    int bt[4], bc[4]; bool bon[4];               // x columns: tap, channel
+// One thread's 8 rows x 4 columns, at(row, column), -> four (per plane) 16-byte units.  ROUND: fp32 to the nearest bf16; otherwise TERMS
+// planes of eight bits each (3: all of an fp32; 1: all of a bf16).
+template <int TERMS, bool ROUND, int PLANE, typename F> __device__ __forceinline__ void wg_put(u32x4* to, int oct, int col, F at) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int jn = n0 + col + j;
-        bon[j] = is_b && jn < Nn;
-        bt[j] = bon[j] ? jn / Cg : 0; bc[j] = bon[j] ? jn - bt[j] * Cg + g * Cg : 0;
+        float c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = at(i, j);
+        const int unit = wg_unit(oct, col + j);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+            if constexpr (ROUND) to[unit] = u32x4{bf16_pack(c[0], c[1]), bf16_pack(c[2], c[3]), bf16_pack(c[4], c[5]), bf16_pack(c[6], c[7])};
+            else to[t * PLANE + unit] = u32x4{top_halves(c[0], c[1]), top_halves(c[2], c[3]), top_halves(c[4], c[5]), top_halves(c[6], c[7])};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] -= bf16_head(c[i]);
+        }
     }
-    const int pad = (p.kernel - 1) * p.dilation / 2;
+}
 
-    f32x16 acc[FM][FN];
+// the matrix instructions of one half (16 rows) of a K step
+template <int TERMS, int PLANE, int FM, int FN>
+__device__ __forceinline__ void wg_mfma(const u32x4* sa, const u32x4* sb, int ks, int wm, int wn, int lane, f32x16 (&acc)[FM][FN]) {
+    bf16x8_t b[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) b[j] = __builtin_bit_cast(bf16x8_t, sb[wg_unit(ks * 2 + (lane >> 5), wn + j * 32 + (lane & 31))]);
+#pragma unroll
+    for (int t = TERMS - 1; t >= 0; --t)          // small terms first
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const bf16x8_t a = __builtin_bit_cast(bf16x8_t, sa[t * PLANE + wg_unit(ks * 2 + (lane >> 5), wm + i * 32 + (lane & 31))]);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
+        }
+}
+
+// element e of a 32 x 32 tile: row 8 * (e / 4) + 4 * (lane / 32) + e % 4, column lane % 32
+template <int FM, int FN>
+__device__ __forceinline__ void wg_store(const Wgrad8Args& p, int splits, int split, int g, int m0, int n0, int lane, const f32x16 (&acc)[FM][FN]) {
+    const int Og = p.O / p.groups, Cg = p.I / p.groups, Nn = p.kernel * Cg;
+    const bool plain = splits > 1 || p.packed;                       // [O, kernel, Cg] slabs / result, or [O, Cg, kernel]
+    float* const out = splits > 1 ? p.ws + (long)split * p.O * Nn : p.dw;
+    const int mine = m0 + 4 * (lane >> 5), left = Og - mine;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = n0 + j * 32 + (lane & 31), t = n / Cg;
+        if (n >= Nn) continue;
+        float* at = out + ((long)g * Og + mine) * Nn + (plain ? n : (n - t * Cg) * p.kernel + t);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i * 32 + e4 * 8 + e < left) at[(long)e * Nn] = acc[i][j][e4 * 4 + e];
+                at += 8L * Nn;
+            }
+    }
+}
+template <int FM, int FN> __device__ __forceinline__ void wg_clear(f32x16 (&acc)[FM][FN]) {
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+}
 
+// Workgroup -> (split, group, tile).  Workgroups go to the eight XCDs in turn; the ones of an XCD get a contiguous run of work, so that
+// the tiles of one split (which read the same rows) share an L2.
+struct WgAt { int split, g, tm, tn; };
+__device__ __forceinline__ WgAt wg_at(int tiles_m, int tiles_n, int groups, int total) {
+    const int per = total >> 3, rem = total & 7, x = blockIdx.x & 7, k = blockIdx.x >> 3;
+    int id = x * per + min(x, rem) + k;
+    WgAt a;
+    a.tn = id % tiles_n; id /= tiles_n;
+    a.tm = id % tiles_m; id /= tiles_m;
+    a.g = id % groups; a.split = id / groups;
+    return a;
+}
+
+// Any width and alignment, any size: element loads, no overlap of loads and products.  128 x 128 x 32, four waves.
+template <typename T, int TERMS>
+__global__ void __launch_bounds__(256) wgrad8_edge_kernel(Wgrad8Args p, int splits, int tiles_m, int tiles_n, int steps_per) {
+    __shared__ u32x4 sa[TERMS * 512];
+    __shared__ u32x4 sb[512];
+    const int Og = p.O / p.groups, Cg = p.I / p.groups, Nn = p.kernel * Cg, nb = (p.I + CK_BLOCK - 1) / CK_BLOCK;
+    const WgAt w = wg_at(tiles_m, tiles_n, p.groups, gridDim.x);
+    const int m0 = w.tm * 128, n0 = w.tn * 128, pad = (p.kernel - 1) * p.dilation / 2;
+    const long R = (long)p.N * p.L, k_begin = (long)w.split * steps_per * WG_BK, k_end = min(R, k_begin + (long)steps_per * WG_BK);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    const bool is_a = tid < 128;
+    const int oct = (tid & 127) >> 5, col = (tid & 31) * 4;
+    int bt[4], bc[4]; bool on[4];                // columns of x: tap, channel
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int jn = (is_a ? m0 : n0) + col + j;
+        on[j] = jn < (is_a ? Og : Nn);
+        bt[j] = is_a || !on[j] ? 0 : jn / Cg; bc[j] = is_a || !on[j] ? 0 : jn - bt[j] * Cg + w.g * Cg;
+    }
+    f32x16 acc[2][2];
+    wg_clear(acc);
     for (long k0 = k_begin; k0 < k_end; k0 += WG_BK) {
         float f[8][4];
         const long r0 = k0 + oct * 8;
-        if (is_a) {
+        int l = (int)(r0 % p.L);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const long r = r0 + i;
-                const T* row = (const T*)p.dy + r * p.O + g * Og + m0 + col;
-                if (VEC && r < k_end && m0 + col < Og) {
-                    if (sizeof(T) == 4) {
-                        const f32x4 v = *reinterpret_cast<const f32x4*>(row);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) f[i][j] = v[j];
-                    } else {
-                        const u32x2 v = *reinterpret_cast<const u32x2*>(row);
-                        f[i][0] = bf16_lo(v[0]); f[i][1] = bf16_hi(v[0]); f[i][2] = bf16_lo(v[1]); f[i][3] = bf16_hi(v[1]);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        f[i][j] = 0.f;
-                        if (!VEC && r < k_end && m0 + col + j < Og) { Raw<T, 1> v; v.load(row + j); v.get(&f[i][j]); }
-                    }
-                }
-            }
-        } else if (is_b) {
-            int l = (int)(r0 % p.L);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const long r = r0 + i;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) f[i][j] = 0.f;
-                if (r < k_end) {
-                    if (VEC) {
-                        const int ls = l + bt[0] * p.dilation - pad;
-                        if (bon[0] && ls >= 0 && ls < p.L) {
-                            const long row = r + bt[0] * p.dilation - pad;
-                            const float s = ck_scale(p.q_code[row * nb + bc[0] / CK_BLOCK]);
-                            Bytes<4> q; q.load(p.q + row * p.I + bc[0]);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) f[i][j] = ck_value(q.get(j), s);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int ls = l + bt[j] * p.dilation - pad;
-                            if (bon[j] && ls >= 0 && ls < p.L) {
-                                const long row = r + bt[j] * p.dilation - pad;
-                                f[i][j] = ck_value((uint8_t)p.q[row * p.I + bc[j]], ck_scale(p.q_code[row * nb + bc[j] / CK_BLOCK]));
-                            }
-                        }
-                    }
-                }
-                l = l + 1 == p.L ? 0 : l + 1;
-            }
-        }
-        __syncthreads();                     // the previous step's fragments have been read
-        if (is_a) {
+        for (int i = 0; i < 8; ++i) {
+            const long r = r0 + i;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int at = wg_unit(oct, col + j);
-                if (TERMS == 1) {
-                    sa[0][at] = u32x4{bf16_pack(f[0][j], f[1][j]), bf16_pack(f[2][j], f[3][j]), bf16_pack(f[4][j], f[5][j]), bf16_pack(f[6][j], f[7][j])};
-                } else {
-#pragma unroll
-                    for (int t = 0; t < TERMS; ++t) {
-                        u32x4 w;
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) w[h] = top_halves(f[2 * h][j], f[2 * h + 1][j]);
-                        sa[t][at] = w;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) f[i][j] -= bf16_head(f[i][j]);
+                float v = 0.f;
+                if (on[j] && r < k_end) {
+                    if (is_a) {
+                        Raw<T, 1> e; e.load((const T*)p.dy + r * p.O + (long)w.g * Og + m0 + col + j); v = e.at(0);
+                    } else {
+                        const long sh = (long)bt[j] * p.dilation - pad, ls = l + sh, row = r + sh;
+                        if (ls >= 0 && ls < p.L) v = ck_value((uint8_t)p.q[row * p.I + bc[j]], ck_scale(p.q_code[row * nb + bc[j] / CK_BLOCK]));
                     }
                 }
+                f[i][j] = v;
             }
-        } else if (is_b) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                sb[wg_unit(oct, col + j)] = u32x4{top_halves(f[0][j], f[1][j]), top_halves(f[2][j], f[3][j]), top_halves(f[4][j], f[5][j]), top_halves(f[6][j], f[7][j])};
+            l = l + 1 == p.L ? 0 : l + 1;
         }
+        __syncthreads();                     // the previous step's fragments have been read
+        const auto at = [&](int i, int j) { return f[i][j]; };
+        if (is_a) wg_put<TERMS, TERMS == 1 && sizeof(T) == 4, 512>(sa, oct, col, at); else wg_put<1, false, 512>(sb, oct, col, at);
         __syncthreads();
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            bf16x8_t b[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j) b[j] = __builtin_bit_cast(bf16x8_t, sb[wg_unit(ks * 2 + (lane >> 5), wn + j * 32 + (lane & 31))]);
-#pragma unroll
-            for (int t = TERMS - 1; t >= 0; --t)          // small terms first
-#pragma unroll
-                for (int i = 0; i < FM; ++i) {
-                    const bf16x8_t a = __builtin_bit_cast(bf16x8_t, sa[t][wg_unit(ks * 2 + (lane >> 5), wm + i * 32 + (lane & 31))]);
-#pragma unroll
-                    for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
-                }
-        }
+        for (int ks = 0; ks < 2; ++ks) wg_mfma<TERMS, 512, 2, 2>(sa, sb, ks, wm, wn, lane, acc);
     }
+    wg_store<2, 2>(p, splits, w.split, w.g, m0 + wm, n0 + wn, lane, acc);
+}
 
-    // element e of a 32 x 32 tile: row 8 * (e / 4) + 4 * (lane / 32) + e % 4, column lane % 32
+// Whole quads of x inside a tap: the pipelined form.  Two LDS stages; while the matrix instructions of step k run, the piece of step
+// k + 1 (its loads were issued a step earlier) is split and stored to the other stage and the loads of step k + 2 are issued: one
+// barrier a step.  The first TM threads stage dy, the other TN threads x, each half of the waves runs its own copy of the loop.
+// Loads go through buffer descriptors of the split's rows, which return zero behind the end; a row outside its sample is sent there.
+template <typename T, int TERMS, int TM, int TN, int WM, int WN>
+__global__ void __launch_bounds__(TM + TN) wgrad8_kernel(Wgrad8Args p, int splits, int tiles_m, int tiles_n, int steps_per) {
+    static_assert((TM / WM) * (TN / WN) * 64 == TM + TN && TM % 64 == 0, "one 8 x 4 piece of an operand tile per thread, whole waves to each operand");
+    constexpr int FM = WM / 32, FN = WN / 32, PLANE = TM * 4, STAGE = TERMS * PLANE + TN * 4;
+    extern __shared__ u32x4 lds[];           // [2][STAGE]
+    const int Og = p.O / p.groups, Cg = p.I / p.groups, Nn = p.kernel * Cg, nb = (p.I + CK_BLOCK - 1) / CK_BLOCK;
+    const WgAt w = wg_at(tiles_m, tiles_n, p.groups, gridDim.x);
+    const int m0 = w.tm * TM, n0 = w.tn * TN, pad = (p.kernel - 1) * p.dilation / 2;
+    const long R = (long)p.N * p.L, k_begin = (long)w.split * steps_per * WG_BK, k_end = min(R, k_begin + (long)steps_per * WG_BK);
+    const int steps = (int)((k_end - k_begin + WG_BK - 1) / WG_BK);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = (wave / (TN / WN)) * WM, wn = (wave % (TN / WN)) * WN;
+    f32x16 acc[FM][FN];
+    wg_clear(acc);
+
+    auto loop = [&](auto load, auto put) {
+        load(0);
+        put(lds);
+        __syncthreads();
+        for (int k = 0; k < steps; ++k) {
+            u32x4* const now = lds + (k & 1) * STAGE;
+            u32x4* const next = lds + ((k & 1) ^ 1) * STAGE;
+            load(k + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            wg_mfma<TERMS, PLANE, FM, FN>(now, now + TERMS * PLANE, 0, wm, wn, lane, acc);
+            __builtin_amdgcn_sched_barrier(0);
+            wg_mfma<TERMS, PLANE, FM, FN>(now, now + TERMS * PLANE, 1, wm, wn, lane, acc);
+            put(next);
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int m = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), n = n0 + wn + j * 32 + (lane & 31);
-                if (m < Og && n < Nn) {
-                    const long o = (long)g * Og + m;
-                    if (splits > 1) p.ws[((long)split * p.O + o) * Nn + n] = acc[i][j][e];
-                    else if (p.packed) p.dw[o * Nn + n] = acc[i][j][e];
-                    else { const int t = n / Cg; p.dw[(o * Cg + n - t * Cg) * p.kernel + t] = acc[i][j][e]; }
-                }
+            for (int i = 0; i < TERMS * FM * FN; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       // a matrix instruction,
+                __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);       // eight vector instructions in its shadow
             }
+            __syncthreads();
+        }
+    };
+    if (wave < TM / 64) {
+        constexpr int SZ = sizeof(T);
+        const int oct = tid / (TM / 4), col = (tid % (TM / 4)) * 4;
+        const long first = (long)w.g * Og + m0;                          // columns behind the group's or the row's end are not stored
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>((const char*)p.dy + (k_begin * p.O + first) * SZ), 0,
+                                                                             (int)(((k_end - k_begin) * p.O - first) * SZ), 0x00020000);
+        const unsigned row = (unsigned)p.O * SZ, base = (unsigned)oct * 8 * row + (unsigned)col * SZ;
+        Raw<T, 4> r[8];
+        loop([&](int k) {
+                 const unsigned at = base + (unsigned)k * WG_BK * row;
+#pragma unroll
+                 for (int i = 0; i < 8; ++i) r[i].load(rs, at + (unsigned)i * row);
+             },
+             [&](u32x4* to) {
+                 wg_put<TERMS, TERMS == 1 && SZ == 4, PLANE>(to, oct, col, [&](int i, int j) { return r[i].at(j); });
+             });
+    } else {
+        const int t2 = tid - TM, oct = t2 / (TN / 4), col = (t2 % (TN / 4)) * 4;
+        const bool on = n0 + col < Nn;
+        const int tap = on ? (n0 + col) / Cg : 0, ch = on ? n0 + col - tap * Cg + w.g * Cg : 0;
+        const int shift = on ? tap * p.dilation - pad : 0x60000000;      // a column that does not exist: never inside a sample
+        const long b0 = max(0L, k_begin - pad), b1 = min(R, k_end - pad + (long)(p.kernel - 1) * p.dilation);
+        const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.q + b0 * p.I), 0, (int)((b1 - b0) * p.I), 0x00020000);
+        const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.q_code + b0 * nb), 0, (int)((b1 - b0) * nb), 0x00020000);
+        const int row0 = (int)(k_begin - b0) + oct * 8 + (on ? shift : 0), step = WG_BK % p.L;
+        unsigned at_q = (unsigned)(row0 * p.I + ch), at_c = (unsigned)(row0 * nb + ch / CK_BLOCK);      // of the next load's first row
+        int l0 = (int)((k_begin + oct * 8) % p.L);                       // and its place in its sample
+        unsigned q[8], c[8];
+        loop([&](int) {
+                 int l = l0;
+#pragma unroll
+                 for (int i = 0; i < 8; ++i) {
+                     const unsigned out = (unsigned)(l + shift) < (unsigned)p.L ? 0u : 0x80000000u;      // behind the end of either buffer
+                     q[i] = __builtin_amdgcn_raw_buffer_load_b32(rq, (at_q + (unsigned)(i * p.I)) | out, 0, 0);
+                     c[i] = __builtin_amdgcn_raw_buffer_load_b8(rc, (at_c + (unsigned)(i * nb)) | out, 0, 0);
+                     l = l + 1 == p.L ? 0 : l + 1;
+                 }
+                 at_q += (unsigned)(WG_BK * p.I); at_c += (unsigned)(WG_BK * nb);
+                 l0 += step;
+                 if (l0 >= p.L) l0 -= p.L;
+             },
+             [&](u32x4* to) {
+                 wg_put<1, false, TN * 4>(to + TERMS * PLANE, oct, col, [&](int i, int j) { return ck_value((q[i] >> (8 * j)) & 0xffu, ck_scale(c[i])); });      // exact
+             });
+    }
+    wg_store<FM, FN>(p, splits, w.split, w.g, m0 + wm, n0 + wn, lane, acc);
 }
 
 // dw = sum over the splits, in split order; [O, kernel, Cg] -> the same (packed) or [O, Cg, kernel]
@@ -195,17 +265,24 @@ __global__ void __launch_bounds__(256) wgrad8_sum_kernel(Wgrad8Args p, int split
     }
 }
 
-struct WgPlan { int tiles_m, tiles_n, splits, steps_per; };
-static WgPlan wg_plan(const Wgrad8Args& p, int TM, int TN) {
+struct WgPlan { int tile, tiles_m, tiles_n, splits, steps_per; bool pipe; };
+static WgPlan wg_plan(const Wgrad8Args& p) {
     WgPlan k;
     const long R = (long)p.N * p.L;
-    const int steps = cdiv(R, WG_BK);
-    k.tiles_m = cdiv(p.O / p.groups, TM); k.tiles_n = cdiv((long)p.kernel * (p.I / p.groups), TN);
-    // enough workgroups for two to a CU, at least eight steps each
-    const long tiles = (long)k.tiles_m * k.tiles_n * p.groups;
-    long want = cdiv(512, tiles);
+    const int Og = p.O / p.groups, Cg = p.I / p.groups, steps = cdiv(R, WG_BK), sz = p.dtype == MTTS_F32 ? 4 : 2;
+    // whole quads of x inside a tap, a bf16 quad of dy at eight bytes; offsets in a split's rows below 2^31
+    k.pipe = Cg % 4 == 0 && aligned_to(p.q, 4) && (sz == 4 || (Og % 4 == 0 && aligned_to(p.dy, 8)));
+    const long span = (long)(p.kernel - 1) * p.dilation + 4 * WG_BK, wide = (long)p.O * sz > p.I ? (long)p.O * sz : p.I;
+    const long most = (((1L << 31) - 1) / wide - span) / WG_BK;          // steps whose offsets fit
+    if (most < 8) k.pipe = false;
+    k.tile = k.pipe && Og > 128 && (long)p.kernel * Cg > 128 ? 256 : 128;
+    k.tiles_m = cdiv(Og, k.tile); k.tiles_n = cdiv((long)p.kernel * Cg, k.tile);
+    // one 256-tile or two 128-tiles to a CU, at least eight steps each
+    const long tiles = (long)k.tiles_m * k.tiles_n * p.groups, room = k.tile == 256 ? 256 : 512;
+    long want = tiles > room ? 1 : room / tiles;
     if (want > steps / 8) want = steps / 8;
     if (want < 1) want = 1;
+    if (k.pipe && cdiv(steps, want) > most) want = cdiv(steps, most);
     k.steps_per = cdiv(steps, want);
     k.splits = cdiv(steps, k.steps_per);
     return k;
@@ -217,25 +294,36 @@ static int wg_check(const Wgrad8Args& p) {
     MTTS_REQUIRE(p.I % p.groups == 0 && p.O % p.groups == 0, "mtts_conv_weight_grad8: %d x %d channels are not a multiple of %d groups", p.I, p.O, p.groups);
     MTTS_REQUIRE(p.dtype == MTTS_F32 || p.dtype == MTTS_BF16, "mtts_conv_weight_grad8: dtype %d is neither MTTS_F32 nor MTTS_BF16", p.dtype);
     MTTS_REQUIRE((long)p.kernel * (p.I / p.groups) < (1L << 28) && (long)(p.kernel - 1) * p.dilation < (1L << 30), "mtts_conv_weight_grad8: kernel %d with dilation %d is too large", p.kernel, p.dilation);
-    const WgPlan k = wg_plan(p, 128, 128);
-    MTTS_REQUIRE((long)k.tiles_m * k.tiles_n * 256 < (1L << 32) && (long)k.splits * p.groups < 65536, "mtts_conv_weight_grad8: too many tiles for one call");
+    const WgPlan k = wg_plan(p);
+    MTTS_REQUIRE((long)k.tiles_m * k.tiles_n * p.groups * k.splits < (1L << 32) / 512, "mtts_conv_weight_grad8: too many tiles for one call");
     return 0;
 }
 
 MTTS_API long mtts_conv_weight_grad8_workspace_floats(const Wgrad8Args* args) {
     if (wg_check(*args)) return -1;
-    const WgPlan k = wg_plan(*args, 128, 128);
+    const WgPlan k = wg_plan(*args);
     return k.splits > 1 ? (long)k.splits * args->O * args->kernel * (args->I / args->groups) : 0;
 }
 
-template <typename T, int TERMS, bool VEC> static void wg_go(const Wgrad8Args& p, hipStream_t s) {
-    const WgPlan k = wg_plan(p, 128, 128);
-    hipLaunchKernelGGL((wgrad8_kernel<T, TERMS, 128, 128, 64, 64, VEC>), dim3(k.tiles_m * k.tiles_n, 1, k.splits * p.groups), dim3(256), 0, s, p, k.splits, k.tiles_n, k.steps_per);
+template <typename T, int TERMS, int TM, int TN, int WM, int WN> static int wg_pipe(const Wgrad8Args& p, const WgPlan& k, hipStream_t s) {
+    const size_t lds = 2 * (TERMS * TM * 4 + TN * 4) * sizeof(u32x4);
+    const void* fn = (const void*)wgrad8_kernel<T, TERMS, TM, TN, WM, WN>;
+    if (lds > 64 * 1024) MTTS_CHECK_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL((wgrad8_kernel<T, TERMS, TM, TN, WM, WN>), dim3(k.tiles_m * k.tiles_n * p.groups * k.splits), dim3(TM + TN), lds, s, p, k.splits, k.tiles_m, k.tiles_n, k.steps_per);
+    return 0;
+}
+template <typename T, int TERMS> static int wg_go(const Wgrad8Args& p, hipStream_t s) {
+    const WgPlan k = wg_plan(p);
+    if (k.pipe && k.tile == 256) MTTS_TRY((wg_pipe<T, TERMS, 256, 256, 64, 128>(p, k, s)));
+    else if (k.pipe) MTTS_TRY((wg_pipe<T, TERMS, 128, 128, 64, 64>(p, k, s)));
+    else hipLaunchKernelGGL((wgrad8_edge_kernel<T, TERMS>), dim3(k.tiles_m * k.tiles_n * p.groups * k.splits), dim3(256), 0, s, p, k.splits, k.tiles_m, k.tiles_n, k.steps_per);
     if (k.splits > 1) {
         const long total = (long)p.O * p.kernel * (p.I / p.groups);
         const long blocks = cdiv(total, 256);
         hipLaunchKernelGGL(wgrad8_sum_kernel, dim3((unsigned)(blocks > 4096 ? 4096 : blocks)), dim3(256), 0, s, p, k.splits);
     }
+    MTTS_CHECK_LAUNCH("conv_weight_grad8");
+    return 0;
 }
 
 MTTS_API int mtts_conv_weight_grad8(const Wgrad8Args* args, void* stream) {
@@ -243,14 +331,7 @@ MTTS_API int mtts_conv_weight_grad8(const Wgrad8Args* args, void* stream) {
     hipStream_t s = (hipStream_t)stream;
     MTTS_TRY(wg_check(p));
     MTTS_REQUIRE(p.q && p.q_code && p.dy && p.dw && (p.ws || mtts_conv_weight_grad8_workspace_floats(&p) == 0), "mtts_conv_weight_grad8: missing tensor");
-    const bool f32 = p.dtype == MTTS_F32;
-    const int Og = p.O / p.groups, Cg = p.I / p.groups;
-    // whole quads of columns inside a group and a tap, at addresses that a quad may start at
-    const bool v = Og % 4 == 0 && Cg % 4 == 0 && aligned_to(p.dy, f32 ? 16 : 8) && aligned_to(p.q, 4);
     const int prec = p.precision ? p.precision : (mtts_get_precision() == 1 ? 1 : 2);      // as GemmArgs.precision
-    if (!f32) v ? wg_go<bf16_t, 1, true>(p, s) : wg_go<bf16_t, 1, false>(p, s);
-    else if (prec == 1) v ? wg_go<float, 1, true>(p, s) : wg_go<float, 1, false>(p, s);
-    else v ? wg_go<float, 3, true>(p, s) : wg_go<float, 3, false>(p, s);
-    MTTS_CHECK_LAUNCH("conv_weight_grad8");
-    return 0;
+    if (p.dtype == MTTS_BF16) return wg_go<bf16_t, 1>(p, s);
+    return prec == 1 ? wg_go<float, 1>(p, s) : wg_go<float, 3>(p, s);
 }
