@@ -246,23 +246,50 @@ __global__ void __launch_bounds__(TM + TN) wgrad8_kernel(Wgrad8Args p, int split
     wg_store<FM, FN>(p, splits, w.split, w.g, m0 + wm, n0 + wn, lane, acc);
 }
 
-// dw = sum over the splits, in split order; [O, kernel, Cg] -> the same (packed) or [O, Cg, kernel]
-__global__ void __launch_bounds__(256) wgrad8_sum_kernel(Wgrad8Args p, int splits) {
-    const int Cg = p.I / p.groups, Nn = p.kernel * Cg;
-    const long total = (long)p.O * Nn, stride = (long)gridDim.x * 256;
-    GridRC rc((long)blockIdx.x * 256 + threadIdx.x, stride, Nn);
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += stride, rc.next()) {
-        float s = 0.f;
-        for (int k0 = 0; k0 < splits; k0 += 8) {
-            float v[8];
+// dw = sum over the splits, in split order; slabs [O, kernel, Cg] -> the same (packed) or [O, Cg, kernel].  A workgroup takes one output
+// channel and CC input channels with all their taps: the sums cross over in LDS, so that reads and writes are both contiguous.
+template <int VEC>
+__global__ void __launch_bounds__(256) wgrad8_sum_kernel(Wgrad8Args p, int splits, int CC, int chunks) {
+    extern __shared__ float tile[];          // [CC][kernel]
+    const int Cg = p.I / p.groups, k = p.kernel, Nn = k * Cg;
+    const int o = blockIdx.x / chunks, c0 = (blockIdx.x - o * chunks) * CC, cc = min(CC, Cg - c0), quads = (cc + VEC - 1) / VEC;
+    const long slab = (long)p.O * Nn;
+    const float* const ws = p.ws + (long)o * Nn + c0;
+    for (int i = threadIdx.x; i < quads * k; i += 256) {
+        const int t = i / quads, c = (i - t * quads) * VEC;
+        float s[VEC];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = p.ws[(long)min(k0 + k, splits - 1) * total + i];
+        for (int j = 0; j < VEC; ++j) s[j] = 0.f;
+        for (int k0 = 0; k0 < splits; k0 += 4) {                         // four slabs requested per round trip, added in slab order
+            Raw<float, VEC> v[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) if (k0 + k < splits) s += v[k];
+            for (int u = 0; u < 4; ++u) v[u].load(ws + min(k0 + u, splits - 1) * slab + (long)t * Cg + c);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (k0 + u < splits)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) s[j] += v[u].at(j);
         }
-        if (p.packed) p.dw[i] = s;
-        else { const int t = rc.col / Cg; p.dw[(rc.row * Cg + rc.col - t * Cg) * p.kernel + t] = s; }
+        if (p.packed) store_vec(p.dw + (long)o * Nn + (long)t * Cg + c0 + c, s);
+        else
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) tile[(c + j) * k + t] = s[j];
     }
+    if (p.packed) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < cc * k; i += 256) p.dw[(long)o * Nn + (long)c0 * k + i] = tile[i];
+}
+static int wg_sum(const Wgrad8Args& p, int splits, hipStream_t s) {
+    const int Cg = p.I / p.groups;
+    int CC = 8192 / p.kernel < 256 ? 8192 / p.kernel : 256;              // at most 32 KB of sums (one channel at least: see wg_check)
+    if (CC >= 4) CC &= ~3;
+    const int chunks = cdiv(Cg, CC);
+    const bool v = Cg % 4 == 0 && CC % 4 == 0 && aligned_to(p.ws, 16) && (!p.packed || aligned_to(p.dw, 16));
+    const size_t lds = p.packed ? 0 : (size_t)CC * p.kernel * 4;
+    const dim3 grid((unsigned)((long)p.O * chunks));
+    if (v) hipLaunchKernelGGL(wgrad8_sum_kernel<4>, grid, dim3(256), lds, s, p, splits, CC, chunks);
+    else hipLaunchKernelGGL(wgrad8_sum_kernel<1>, grid, dim3(256), lds, s, p, splits, CC, chunks);
+    return 0;
 }
 
 struct WgPlan { int tile, tiles_m, tiles_n, splits, steps_per; bool pipe; };
@@ -294,6 +321,7 @@ static int wg_check(const Wgrad8Args& p) {
     MTTS_REQUIRE(p.I % p.groups == 0 && p.O % p.groups == 0, "mtts_conv_weight_grad8: %d x %d channels are not a multiple of %d groups", p.I, p.O, p.groups);
     MTTS_REQUIRE(p.dtype == MTTS_F32 || p.dtype == MTTS_BF16, "mtts_conv_weight_grad8: dtype %d is neither MTTS_F32 nor MTTS_BF16", p.dtype);
     MTTS_REQUIRE((long)p.kernel * (p.I / p.groups) < (1L << 28) && (long)(p.kernel - 1) * p.dilation < (1L << 30), "mtts_conv_weight_grad8: kernel %d with dilation %d is too large", p.kernel, p.dilation);
+    MTTS_REQUIRE(p.kernel <= 8192 && (long)p.O * (p.I / p.groups) < (1L << 32) / 256, "mtts_conv_weight_grad8: %d output x %d input channels of %d taps are too many for one call", p.O, p.I / p.groups, p.kernel);
     const WgPlan k = wg_plan(p);
     MTTS_REQUIRE((long)k.tiles_m * k.tiles_n * p.groups * k.splits < (1L << 32) / 512, "mtts_conv_weight_grad8: too many tiles for one call");
     return 0;
@@ -317,11 +345,7 @@ template <typename T, int TERMS> static int wg_go(const Wgrad8Args& p, hipStream
     if (k.pipe && k.tile == 256) MTTS_TRY((wg_pipe<T, TERMS, 256, 256, 64, 128>(p, k, s)));
     else if (k.pipe) MTTS_TRY((wg_pipe<T, TERMS, 128, 128, 64, 64>(p, k, s)));
     else hipLaunchKernelGGL((wgrad8_edge_kernel<T, TERMS>), dim3(k.tiles_m * k.tiles_n * p.groups * k.splits), dim3(256), 0, s, p, k.splits, k.tiles_m, k.tiles_n, k.steps_per);
-    if (k.splits > 1) {
-        const long total = (long)p.O * p.kernel * (p.I / p.groups);
-        const long blocks = cdiv(total, 256);
-        hipLaunchKernelGGL(wgrad8_sum_kernel, dim3((unsigned)(blocks > 4096 ? 4096 : blocks)), dim3(256), 0, s, p, k.splits);
-    }
+    if (k.splits > 1) MTTS_TRY(wg_sum(p, k.splits, s));
     MTTS_CHECK_LAUNCH("conv_weight_grad8");
     return 0;
 }
