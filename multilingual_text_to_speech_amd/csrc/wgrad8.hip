@@ -8,6 +8,10 @@
 // the leading eight bits of what is left (an exact split, 24 bits), against six where both operands are fp32.  fp32 accumulation.
 // A bf16 gradient, and an fp32 one in bf16 mode (rounded to nearest even), takes one term.
 //
+// What bounds it: the matrix pipes.  At 38400 rows, 512 -> 512 channels, kernel 5 (100.7 GFLOP, three terms) the whole call takes 248 us,
+// 1220 TFLOP/s of bf16 products where a plain bf16 library product of 8192^3 reaches 1330 on the same card; with a bf16 gradient 163 us.
+// At 7680 rows, bf16 (20 GFLOP) 48 us: a third of that is the partial tiles' way through memory (63 MB out and in at twelve splits).
+//
 // Tile TM x TN x 32 rows per workgroup, v_mfma_f32_32x32x16_bf16.  A thread takes 8 rows x 4 columns: the transposition happens in
 // registers, and 8 rows of one column are the 16 bytes that a lane feeds to the matrix instruction.  LDS holds these 16-byte units in
 // fragment order, [32-column block][row octet][column], the column XORed with (column / 8) & 3 so that the stores (four columns per
@@ -302,13 +306,21 @@ static WgPlan wg_plan(const Wgrad8Args& p) {
     const long span = (long)(p.kernel - 1) * p.dilation + 4 * WG_BK, wide = (long)p.O * sz > p.I ? (long)p.O * sz : p.I;
     const long most = (((1L << 31) - 1) / wide - span) / WG_BK;          // steps whose offsets fit
     if (most < 8) k.pipe = false;
-    k.tile = k.pipe && Og > 128 && (long)p.kernel * Cg > 128 ? 256 : 128;
-    k.tiles_m = cdiv(Og, k.tile); k.tiles_n = cdiv((long)p.kernel * Cg, k.tile);
-    // one 256-tile or two 128-tiles to a CU, at least eight steps each
-    const long tiles = (long)k.tiles_m * k.tiles_n * p.groups, room = k.tile == 256 ? 256 : 512;
-    long want = tiles > room ? 1 : room / tiles;
-    if (want > steps / 8) want = steps / 8;
-    if (want < 1) want = 1;
+    const long Nn = (long)p.kernel * Cg;
+    auto tiles = [&](long t) { return cdiv(Og, t) * (long)cdiv(Nn, t) * p.groups; };
+    auto split = [&](long t, long room) {        // `room` workgroups fill the card; at least eight steps each
+        long want = tiles(t) > room ? 1 : room / tiles(t);
+        if (want > steps / 8) want = steps / 8;
+        return want < 1 ? 1 : want;
+    };
+    // 256 x 256 tiles (one to a CU) where they fill three quarters of the CUs and waste less than 0.3 of their area, 128 x 128 (two to a
+    // CU) elsewhere.  Rows, I -> O, kernel, fp32 gradients, 256 / 128, us: 38400, 512 -> 512, 5: 294 / 326; 7680: 70 / 76;
+    // 38400, kernel 1: 71 / 75; 960 (60 workgroups): 39 / 26; 38400, 256 -> 256, 1 (150 workgroups): 44 / 38; 14400, 128 -> 320, 5
+    // (0.52 of the area used): 43 / 37; 38400, 512 -> 80, 5: 130 / 90
+    const bool big = k.pipe && tiles(256) * split(256, 256) >= 192 && 10.0 * Og * Nn >= 7.0 * 65536 * (double)(tiles(256) / p.groups);
+    k.tile = big ? 256 : 128;
+    k.tiles_m = cdiv(Og, k.tile); k.tiles_n = cdiv(Nn, k.tile);
+    long want = big ? split(256, 256) : split(128, 512);
     if (k.pipe && cdiv(steps, want) > most) want = cdiv(steps, most);
     k.steps_per = cdiv(steps, want);
     k.splits = cdiv(steps, k.steps_per);

@@ -284,7 +284,8 @@ def check_weight_grad(held, dy, k, d=1, g=1, rounded=False):
 # tile, groups that start inside a block, many rows (split), wide outputs
 GRADS = [(1, 1, 4, 4, 1, 1, 1), (1, 1, 64, 32, 5, 1, 1), (3, 2, 32, 64, 5, 1, 1), (2, 9, 80, 512, 5, 1, 1), (7, 211, 80, 96, 5, 1, 1), (4, 31, 37, 21, 3, 2, 1),
          (3, 50, 60, 36, 3, 9, 3), (2, 40, 70, 30, 7, 3, 5), (5, 133, 640, 320, 3, 9, 5), (16, 120, 512, 512, 5, 1, 1), (2, 700, 256, 130, 1, 1, 1),
-         (64, 600, 32, 64, 3, 1, 1), (1, 5000, 100, 100, 2, 1, 1), (3, 17, 48, 48, 4, 3, 1), (2, 12, 64, 64, 31, 5, 1), (2, 100, 1040, 260, 1, 1, 2)]
+         (64, 600, 32, 64, 3, 1, 1), (1, 5000, 100, 100, 2, 1, 1), (3, 17, 48, 48, 4, 3, 1), (2, 12, 64, 64, 31, 5, 1), (2, 100, 1040, 260, 1, 1, 2),
+         (40, 200, 128, 256, 5, 1, 1), (33, 301, 256, 260, 3, 2, 1), (2, 400, 8, 8, 2500, 1, 1)]
 
 
 @pytest.mark.parametrize('dtype', [F32, BF16])
