@@ -31,11 +31,9 @@ __global__ void __launch_bounds__(CK_T) ck_pack_kernel(const T* __restrict__ x, 
         }
 #pragma unroll
         for (int u = 0; u < CK_U; ++u) {
-            float f[VEC];
-            get_vec(v[u], f);
             unsigned m = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) m = umax_(m, abs_bits(f[j]));
+            for (int j = 0; j < VEC; ++j) m = umax_(m, abs_bits(v[u].at(j)));
             if (VEC == 1) {
 #pragma unroll
                 for (int d = 1; d < CK_BLOCK; d *= 2) m = umax_(m, (unsigned)__shfl_xor((int)m, d, 64));
@@ -46,18 +44,8 @@ __global__ void __launch_bounds__(CK_T) ck_pack_kernel(const T* __restrict__ x, 
             if (in[u]) {
                 const long at = row0 + row[u];
                 if (col[u] < C) {
-                    if (VEC == 1) q[at * C + col[u]] = (int8_t)ck_quantise(f[0], c);
-                    else {
-                        unsigned w[VEC > 4 ? 2 : 1];
-#pragma unroll
-                        for (int h = 0; h < (VEC > 4 ? 2 : 1); ++h) {
-                            w[h] = 0;
-#pragma unroll
-                            for (int j = 0; j < 4 && 4 * h + j < VEC; ++j) w[h] |= ((unsigned)ck_quantise(f[4 * h + j], c) & 0xffu) << (8 * j);
-                        }
-                        if (VEC == 4) *reinterpret_cast<unsigned*>(q + at * C + col[u]) = w[0];
-                        else *reinterpret_cast<u32x2*>(q + at * C + col[u]) = u32x2{w[0], w[VEC > 4 ? 1 : 0]};
-                    }
+                    if constexpr (VEC == 1) q[at * C + col[u]] = (int8_t)ck_quantise(v[u].at(0), c);
+                    else ck_store(q + at * C + col[u], v[u], c);
                 }
                 if ((col[u] & (CK_BLOCK - 1)) == 0) code[at * nb + col[u] / CK_BLOCK] = (uint8_t)c;
             }

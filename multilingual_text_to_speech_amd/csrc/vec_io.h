@@ -36,6 +36,7 @@ template <> struct Raw<bf16_t, 4> {
 template <> struct Raw<bf16_t, 8> {
     u32x4 w;
     __device__ __forceinline__ void load(const bf16_t* p) { w = *reinterpret_cast<const u32x4*>(p); }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned at) { w = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0); }
     __device__ __forceinline__ float at(int j) const { return j & 1 ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]); }
     __device__ __forceinline__ void zero() { w = u32x4{0, 0, 0, 0}; }
 };
@@ -62,6 +63,12 @@ __device__ __forceinline__ void store_vec(float* p, const float (&f)[1]) { *p = 
 __device__ __forceinline__ void store_vec(bf16_t* p, const float (&f)[8]) {
     *reinterpret_cast<u32x4*>(p) = u32x4{bf16_pack(f[0], f[1]), bf16_pack(f[2], f[3]), bf16_pack(f[4], f[5]), bf16_pack(f[6], f[7])};
 }
+__device__ __forceinline__ void store_vec(__amdgpu_buffer_rsrc_t r, unsigned at, const float (&f)[4]) {
+    __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])}, r, at, 0, 0);
+}
+__device__ __forceinline__ void store_vec(__amdgpu_buffer_rsrc_t r, unsigned at, const float (&f)[8]) {
+    __builtin_amdgcn_raw_buffer_store_b128(u32x4{bf16_pack(f[0], f[1]), bf16_pack(f[2], f[3]), bf16_pack(f[4], f[5]), bf16_pack(f[6], f[7])}, r, at, 0, 0);
+}
 __device__ __forceinline__ void store_vec(bf16_t* p, const float (&f)[1]) { p->v = (uint16_t)bf16_pack(f[0], 0.f); }
 
 // VEC bytes (8-bit values, keep flags)
@@ -75,12 +82,14 @@ template <> struct Bytes<1> {
 template <> struct Bytes<4> {
     unsigned w;
     __device__ __forceinline__ void load(const void* p) { w = *(const unsigned*)p; }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned at) { w = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0); }
     __device__ __forceinline__ unsigned get(int j) const { return (w >> (8 * j)) & 0xffu; }
     __device__ __forceinline__ void fill(unsigned v) { w = v * 0x01010101u; }
 };
 template <> struct Bytes<8> {
     u32x2 w;
     __device__ __forceinline__ void load(const void* p) { w = *(const u32x2*)p; }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned at) { w = __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0); }
     __device__ __forceinline__ unsigned get(int j) const { return (w[j >> 2] >> (8 * (j & 3))) & 0xffu; }
     __device__ __forceinline__ void fill(unsigned v) { w = u32x2{v * 0x01010101u, v * 0x01010101u}; }
 };
@@ -102,6 +111,21 @@ __device__ __forceinline__ int ck_quantise(float x, unsigned code) {
     const float inv = __uint_as_float((254u - code) << 23);          // 2^(127 - code): exact for code <= 249
     const float top = code == 249u ? 63.f : 127.f;
     return (int)fminf(fmaxf(rintf(x * inv), -top), top);
+}
+// four (h = 0) or eight values of a vector, as bytes
+template <typename R> __device__ __forceinline__ unsigned ck_word(const R& x, int h, unsigned code) {
+    unsigned w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w |= ((unsigned)ck_quantise(x.at(4 * h + j), code) & 0xffu) << (8 * j);
+    return w;
+}
+__device__ __forceinline__ void ck_store(int8_t* q, const Raw<float, 4>& x, unsigned code) { *reinterpret_cast<unsigned*>(q) = ck_word(x, 0, code); }
+__device__ __forceinline__ void ck_store(int8_t* q, const Raw<bf16_t, 8>& x, unsigned code) { *reinterpret_cast<u32x2*>(q) = u32x2{ck_word(x, 0, code), ck_word(x, 1, code)}; }
+__device__ __forceinline__ void ck_store(__amdgpu_buffer_rsrc_t r, unsigned at, const Raw<float, 4>& x, unsigned code) {
+    __builtin_amdgcn_raw_buffer_store_b32(ck_word(x, 0, code), r, at, 0, 0);
+}
+__device__ __forceinline__ void ck_store(__amdgpu_buffer_rsrc_t r, unsigned at, const Raw<bf16_t, 8>& x, unsigned code) {
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{ck_word(x, 0, code), ck_word(x, 1, code)}, r, at, 0, 0);
 }
 __device__ __forceinline__ float ck_scale(unsigned code) { return __uint_as_float(code << 23); }      // 255: infinity
 __device__ __forceinline__ float ck_value(unsigned byte, float scale) { return (float)(int)(int8_t)byte * scale; }
