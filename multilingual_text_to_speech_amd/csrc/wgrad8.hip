@@ -64,18 +64,28 @@ __device__ __forceinline__ void wg_mfma(const u32x4* sa, const u32x4* sb, int ks
         }
 }
 
+// Columns of the product: per tap, the quads of channels (at whole multiples of four, so that a quad lies in one checkpoint block) that
+// touch the group: Cp = quad columns, the first one at channel `first`; the channels of other groups in the outer quads are not stored.
+struct WgCols { int Cp, first, skip; };
+__host__ __device__ inline int wg_quad_columns(int Cg) { return Cg % 4 == 0 ? Cg : ((Cg + 6) & ~3); }
+__device__ __forceinline__ WgCols wg_cols(const Wgrad8Args& p, int g) {
+    const int Cg = p.I / p.groups;
+    return WgCols{wg_quad_columns(Cg), g * Cg & ~3, g * Cg & 3};
+}
+
 // element e of a 32 x 32 tile: row 8 * (e / 4) + 4 * (lane / 32) + e % 4, column lane % 32
 template <int FM, int FN>
 __device__ __forceinline__ void wg_store(const Wgrad8Args& p, int splits, int split, int g, int m0, int n0, int lane, const f32x16 (&acc)[FM][FN]) {
     const int Og = p.O / p.groups, Cg = p.I / p.groups, Nn = p.kernel * Cg;
+    const WgCols cols = wg_cols(p, g);
     const bool plain = splits > 1 || p.packed;                       // [O, kernel, Cg] slabs / result, or [O, Cg, kernel]
     float* const out = splits > 1 ? p.ws + (long)split * p.O * Nn : p.dw;
     const int mine = m0 + 4 * (lane >> 5), left = Og - mine;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-        const int n = n0 + j * 32 + (lane & 31), t = n / Cg;
-        if (n >= Nn) continue;
-        float* at = out + ((long)g * Og + mine) * Nn + (plain ? n : (n - t * Cg) * p.kernel + t);
+        const int n = n0 + j * 32 + (lane & 31), t = n / cols.Cp, c = n - t * cols.Cp - cols.skip;
+        if (t >= p.kernel || c < 0 || c >= Cg) continue;
+        float* at = out + ((long)g * Og + mine) * Nn + (plain ? t * Cg + c : c * p.kernel + t);
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -109,13 +119,14 @@ __device__ __forceinline__ WgAt wg_at(int tiles_m, int tiles_n, int groups, int 
     return a;
 }
 
-// Any width and alignment, any size: element loads, no overlap of loads and products.  128 x 128 x 32, four waves.
+// Any size (dilations whose offsets pass 2^31): element loads, no overlap of loads and products.  128 x 128 x 32, four waves.
 template <typename T, int TERMS>
 __global__ void __launch_bounds__(256) wgrad8_edge_kernel(Wgrad8Args p, int splits, int tiles_m, int tiles_n, int steps_per) {
     __shared__ u32x4 sa[TERMS * 512];
     __shared__ u32x4 sb[512];
-    const int Og = p.O / p.groups, Cg = p.I / p.groups, Nn = p.kernel * Cg, nb = (p.I + CK_BLOCK - 1) / CK_BLOCK;
+    const int Og = p.O / p.groups, nb = (p.I + CK_BLOCK - 1) / CK_BLOCK;
     const WgAt w = wg_at(tiles_m, tiles_n, p.groups, gridDim.x);
+    const WgCols cols = wg_cols(p, w.g);
     const int m0 = w.tm * 128, n0 = w.tn * 128, pad = (p.kernel - 1) * p.dilation / 2;
     const long R = (long)p.N * p.L, k_begin = (long)w.split * steps_per * WG_BK, k_end = min(R, k_begin + (long)steps_per * WG_BK);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
@@ -125,8 +136,9 @@ __global__ void __launch_bounds__(256) wgrad8_edge_kernel(Wgrad8Args p, int spli
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int jn = (is_a ? m0 : n0) + col + j;
-        on[j] = jn < (is_a ? Og : Nn);
-        bt[j] = is_a || !on[j] ? 0 : jn / Cg; bc[j] = is_a || !on[j] ? 0 : jn - bt[j] * Cg + w.g * Cg;
+        on[j] = jn < (is_a ? Og : p.kernel * cols.Cp);
+        bt[j] = is_a || !on[j] ? 0 : jn / cols.Cp; bc[j] = is_a || !on[j] ? 0 : jn - bt[j] * cols.Cp + cols.first;
+        if (bc[j] >= p.I) on[j] = false;
     }
     f32x16 acc[2][2];
     wg_clear(acc);
@@ -162,16 +174,17 @@ __global__ void __launch_bounds__(256) wgrad8_edge_kernel(Wgrad8Args p, int spli
     wg_store<2, 2>(p, splits, w.split, w.g, m0 + wm, n0 + wn, lane, acc);
 }
 
-// Whole quads of x inside a tap: the pipelined form.  Two LDS stages; while the matrix instructions of step k run, the piece of step
+// The pipelined form.  Two LDS stages; while the matrix instructions of step k run, the piece of step
 // k + 1 (its loads were issued a step earlier) is split and stored to the other stage and the loads of step k + 2 are issued: one
 // barrier a step.  The first TM threads stage dy, the other TN threads x, each half of the waves runs its own copy of the loop.
 // Loads go through buffer descriptors of the split's rows, which return zero behind the end; a row outside its sample is sent there.
-template <typename T, int TERMS, int TM, int TN, int WM, int WN>
+// ODD: quads of x or of a bf16 dy may start at any byte; the aligned words around them are loaded and shifted together.
+template <typename T, int TERMS, int TM, int TN, int WM, int WN, bool ODD>
 __global__ void __launch_bounds__(TM + TN) wgrad8_kernel(Wgrad8Args p, int splits, int tiles_m, int tiles_n, int steps_per) {
     static_assert((TM / WM) * (TN / WN) * 64 == TM + TN && TM % 64 == 0, "one 8 x 4 piece of an operand tile per thread, whole waves to each operand");
     constexpr int FM = WM / 32, FN = WN / 32, PLANE = TM * 4, STAGE = TERMS * PLANE + TN * 4;
     extern __shared__ u32x4 lds[];           // [2][STAGE]
-    const int Og = p.O / p.groups, Cg = p.I / p.groups, Nn = p.kernel * Cg, nb = (p.I + CK_BLOCK - 1) / CK_BLOCK;
+    const int Og = p.O / p.groups, nb = (p.I + CK_BLOCK - 1) / CK_BLOCK;
     const WgAt w = wg_at(tiles_m, tiles_n, p.groups, gridDim.x);
     const int m0 = w.tm * TM, n0 = w.tn * TN, pad = (p.kernel - 1) * p.dilation / 2;
     const long R = (long)p.N * p.L, k_begin = (long)w.split * steps_per * WG_BK, k_end = min(R, k_begin + (long)steps_per * WG_BK);
@@ -206,36 +219,58 @@ __global__ void __launch_bounds__(TM + TN) wgrad8_kernel(Wgrad8Args p, int split
         constexpr int SZ = sizeof(T);
         const int oct = tid / (TM / 4), col = (tid % (TM / 4)) * 4;
         const long first = (long)w.g * Og + m0;                          // columns behind the group's or the row's end are not stored
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>((const char*)p.dy + (k_begin * p.O + first) * SZ), 0,
-                                                                             (int)(((k_end - k_begin) * p.O - first) * SZ), 0x00020000);
-        const unsigned row = (unsigned)p.O * SZ, base = (unsigned)oct * 8 * row + (unsigned)col * SZ;
-        Raw<T, 4> r[8];
-        loop([&](int k) {
-                 const unsigned at = base + (unsigned)k * WG_BK * row;
+        const char* const from = (const char*)p.dy + (k_begin * p.O + first) * SZ;
+        const unsigned lead = ODD && SZ == 2 ? (unsigned)((uintptr_t)from & 3) : 0u;      // descriptors start at a whole word
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(from) - lead, 0, (int)((((k_end - k_begin) * p.O - first) * SZ + lead + 3) & ~3L), 0x00020000);
+        const unsigned row = (unsigned)p.O * SZ, base = (unsigned)oct * 8 * row + (unsigned)col * SZ + lead;
+        if constexpr (ODD && SZ == 2) {
+            u32x3 r[8]; unsigned odd[8];
+            loop([&](int k) {
+                     const unsigned at = base + (unsigned)k * WG_BK * row;
 #pragma unroll
-                 for (int i = 0; i < 8; ++i) r[i].load(rs, at + (unsigned)i * row);
-             },
-             [&](u32x4* to) {
-                 wg_put<TERMS, TERMS == 1 && SZ == 4, PLANE>(to, oct, col, [&](int i, int j) { return r[i].at(j); });
-             });
+                     for (int i = 0; i < 8; ++i) { const unsigned o = at + (unsigned)i * row; odd[i] = o & 2; r[i] = __builtin_amdgcn_raw_buffer_load_b96(rs, o & ~3u, 0, 0); }
+                 },
+                 [&](u32x4* to) {
+                     wg_put<1, false, PLANE>(to, oct, col, [&](int i, int j) {
+                         const unsigned w = __builtin_amdgcn_alignbyte(r[i][(j >> 1) + 1], r[i][j >> 1], odd[i]);
+                         return j & 1 ? bf16_hi(w) : bf16_lo(w);
+                     });
+                 });
+        } else {
+            Raw<T, 4> r[8];
+            loop([&](int k) {
+                     const unsigned at = base + (unsigned)k * WG_BK * row;
+#pragma unroll
+                     for (int i = 0; i < 8; ++i) r[i].load(rs, at + (unsigned)i * row);
+                 },
+                 [&](u32x4* to) {
+                     wg_put<TERMS, TERMS == 1 && SZ == 4, PLANE>(to, oct, col, [&](int i, int j) { return r[i].at(j); });
+                 });
+        }
     } else {
         const int t2 = tid - TM, oct = t2 / (TN / 4), col = (t2 % (TN / 4)) * 4;
-        const bool on = n0 + col < Nn;
-        const int tap = on ? (n0 + col) / Cg : 0, ch = on ? n0 + col - tap * Cg + w.g * Cg : 0;
+        const WgCols cols = wg_cols(p, w.g);
+        const int tap = (n0 + col) / cols.Cp, ch = n0 + col - tap * cols.Cp + cols.first;
+        const bool on = tap < p.kernel && ch < p.I;
         const int shift = on ? tap * p.dilation - pad : 0x60000000;      // a column that does not exist: never inside a sample
         const long b0 = max(0L, k_begin - pad), b1 = min(R, k_end - pad + (long)(p.kernel - 1) * p.dilation);
-        const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.q + b0 * p.I), 0, (int)((b1 - b0) * p.I), 0x00020000);
+        const int8_t* const from = p.q + b0 * p.I;
+        const unsigned lead = ODD ? (unsigned)((uintptr_t)from & 3) : 0u;
+        const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(from) - lead, 0, (int)(((b1 - b0) * p.I + lead + 3) & ~3L), 0x00020000);
         const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.q_code + b0 * nb), 0, (int)((b1 - b0) * nb), 0x00020000);
         const int row0 = (int)(k_begin - b0) + oct * 8 + (on ? shift : 0), step = WG_BK % p.L;
-        unsigned at_q = (unsigned)(row0 * p.I + ch), at_c = (unsigned)(row0 * nb + ch / CK_BLOCK);      // of the next load's first row
+        unsigned at_q = (unsigned)(row0 * p.I + ch) + lead, at_c = (unsigned)(row0 * nb + ch / CK_BLOCK);      // of the next load's first row
         int l0 = (int)((k_begin + oct * 8) % p.L);                       // and its place in its sample
         unsigned q[8], c[8];
+        u32x2 wide[ODD ? 8 : 1];
         loop([&](int) {
                  int l = l0;
 #pragma unroll
                  for (int i = 0; i < 8; ++i) {
                      const unsigned out = (unsigned)(l + shift) < (unsigned)p.L ? 0u : 0x80000000u;      // behind the end of either buffer
-                     q[i] = __builtin_amdgcn_raw_buffer_load_b32(rq, (at_q + (unsigned)(i * p.I)) | out, 0, 0);
+                     const unsigned o = at_q + (unsigned)(i * p.I);
+                     if constexpr (ODD) { wide[i] = __builtin_amdgcn_raw_buffer_load_b64(rq, (o & ~3u) | out, 0, 0); q[i] = o; }
+                     else q[i] = __builtin_amdgcn_raw_buffer_load_b32(rq, o | out, 0, 0);
                      c[i] = __builtin_amdgcn_raw_buffer_load_b8(rc, (at_c + (unsigned)(i * nb)) | out, 0, 0);
                      l = l + 1 == p.L ? 0 : l + 1;
                  }
@@ -244,6 +279,9 @@ __global__ void __launch_bounds__(TM + TN) wgrad8_kernel(Wgrad8Args p, int split
                  if (l0 >= p.L) l0 -= p.L;
              },
              [&](u32x4* to) {
+                 if constexpr (ODD)
+#pragma unroll
+                     for (int i = 0; i < 8; ++i) q[i] = __builtin_amdgcn_alignbyte(wide[i][1], wide[i][0], q[i]);
                  wg_put<1, false, TN * 4>(to + TERMS * PLANE, oct, col, [&](int i, int j) { return ck_value((q[i] >> (8 * j)) & 0xffu, ck_scale(c[i])); });      // exact
              });
     }
@@ -296,17 +334,18 @@ static int wg_sum(const Wgrad8Args& p, int splits, hipStream_t s) {
     return 0;
 }
 
-struct WgPlan { int tile, tiles_m, tiles_n, splits, steps_per; bool pipe; };
+struct WgPlan { int tile, tiles_m, tiles_n, splits, steps_per; bool pipe, odd; };
 static WgPlan wg_plan(const Wgrad8Args& p) {
     WgPlan k;
     const long R = (long)p.N * p.L;
     const int Og = p.O / p.groups, Cg = p.I / p.groups, steps = cdiv(R, WG_BK), sz = p.dtype == MTTS_F32 ? 4 : 2;
-    // whole quads of x inside a tap, a bf16 quad of dy at eight bytes; offsets in a split's rows below 2^31
-    k.pipe = Cg % 4 == 0 && aligned_to(p.q, 4) && (sz == 4 || (Og % 4 == 0 && aligned_to(p.dy, 8)));
+    // quads of x and of a bf16 dy at whole words
+    k.odd = p.I % 4 != 0 || !aligned_to(p.q, 4) || (sz == 2 && (p.O % 4 != 0 || Og % 4 != 0 || !aligned_to(p.dy, 8)));
+    k.pipe = true;                               // offsets in a split's rows below 2^31
     const long span = (long)(p.kernel - 1) * p.dilation + 4 * WG_BK, wide = (long)p.O * sz > p.I ? (long)p.O * sz : p.I;
-    const long most = (((1L << 31) - 1) / wide - span) / WG_BK;          // steps whose offsets fit
+    const long most = (((1L << 31) - 8) / wide - span) / WG_BK;          // steps whose offsets fit
     if (most < 8) k.pipe = false;
-    const long Nn = (long)p.kernel * Cg;
+    const long Nn = (long)p.kernel * wg_quad_columns(Cg);
     auto tiles = [&](long t) { return cdiv(Og, t) * (long)cdiv(Nn, t) * p.groups; };
     auto split = [&](long t, long room) {        // `room` workgroups fill the card; at least eight steps each
         long want = tiles(t) > room ? 1 : room / tiles(t);
@@ -345,12 +384,15 @@ MTTS_API long mtts_conv_weight_grad8_workspace_floats(const Wgrad8Args* args) {
     return k.splits > 1 ? (long)k.splits * args->O * args->kernel * (args->I / args->groups) : 0;
 }
 
-template <typename T, int TERMS, int TM, int TN, int WM, int WN> static int wg_pipe(const Wgrad8Args& p, const WgPlan& k, hipStream_t s) {
+template <typename T, int TERMS, int TM, int TN, int WM, int WN, bool ODD> static int wg_launch(const Wgrad8Args& p, const WgPlan& k, hipStream_t s) {
     const size_t lds = 2 * (TERMS * TM * 4 + TN * 4) * sizeof(u32x4);
-    const void* fn = (const void*)wgrad8_kernel<T, TERMS, TM, TN, WM, WN>;
+    const void* fn = (const void*)wgrad8_kernel<T, TERMS, TM, TN, WM, WN, ODD>;
     if (lds > 64 * 1024) MTTS_CHECK_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL((wgrad8_kernel<T, TERMS, TM, TN, WM, WN>), dim3(k.tiles_m * k.tiles_n * p.groups * k.splits), dim3(TM + TN), lds, s, p, k.splits, k.tiles_m, k.tiles_n, k.steps_per);
+    hipLaunchKernelGGL((wgrad8_kernel<T, TERMS, TM, TN, WM, WN, ODD>), dim3(k.tiles_m * k.tiles_n * p.groups * k.splits), dim3(TM + TN), lds, s, p, k.splits, k.tiles_m, k.tiles_n, k.steps_per);
     return 0;
+}
+template <typename T, int TERMS, int TM, int TN, int WM, int WN> static int wg_pipe(const Wgrad8Args& p, const WgPlan& k, hipStream_t s) {
+    return k.odd ? wg_launch<T, TERMS, TM, TN, WM, WN, true>(p, k, s) : wg_launch<T, TERMS, TM, TN, WM, WN, false>(p, k, s);
 }
 template <typename T, int TERMS> static int wg_go(const Wgrad8Args& p, hipStream_t s) {
     const WgPlan k = wg_plan(p);

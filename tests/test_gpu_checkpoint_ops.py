@@ -285,7 +285,8 @@ def check_weight_grad(held, dy, k, d=1, g=1, rounded=False):
 GRADS = [(1, 1, 4, 4, 1, 1, 1), (1, 1, 64, 32, 5, 1, 1), (3, 2, 32, 64, 5, 1, 1), (2, 9, 80, 512, 5, 1, 1), (7, 211, 80, 96, 5, 1, 1), (4, 31, 37, 21, 3, 2, 1),
          (3, 50, 60, 36, 3, 9, 3), (2, 40, 70, 30, 7, 3, 5), (5, 133, 640, 320, 3, 9, 5), (16, 120, 512, 512, 5, 1, 1), (2, 700, 256, 130, 1, 1, 1),
          (64, 600, 32, 64, 3, 1, 1), (1, 5000, 100, 100, 2, 1, 1), (3, 17, 48, 48, 4, 3, 1), (2, 12, 64, 64, 31, 5, 1), (2, 100, 1040, 260, 1, 1, 2),
-         (40, 200, 128, 256, 5, 1, 1), (33, 301, 256, 260, 3, 2, 1), (2, 400, 8, 8, 2500, 1, 1)]
+         (40, 200, 128, 256, 5, 1, 1), (33, 301, 256, 260, 3, 2, 1), (2, 400, 8, 8, 2500, 1, 1),
+         (33, 301, 257, 259, 3, 2, 1), (20, 400, 130, 514, 5, 1, 2), (8, 99, 505, 307, 3, 1, 1), (1, 5, 3, 2, 3, 1, 1), (1, 5, 512, 8, 3, 1 << 22, 1), (3, 100, 35, 70, 5, 1, 7)]
 
 
 @pytest.mark.parametrize('dtype', [F32, BF16])
@@ -329,6 +330,9 @@ def test_weight_grad_of_strided_and_misaligned_operands():
     v.copy_(held.values)
     assert torch.equal(K.conv1d_weight_grad8(held, dy.transpose(0, 1).contiguous().transpose(0, 1), 3), want)
     check_weight_grad(K.Checkpoint8(v, held.scales), o, 3)
+    half = torch.empty(dy.numel() + 1, dtype=BF16, device=DEV)[1:].view_as(dy)
+    half.copy_(dy)
+    check_weight_grad(K.Checkpoint8(v, held.scales), half, 3)
 
 
 def test_weight_grad_of_no_rows_and_of_a_lost_block():
