@@ -143,7 +143,7 @@ typedef struct GroupNormArgs {
     float* rstd;
     int8_t* q;             /* [N, L, C] 8-bit checkpoint of x: written by fwd, read by bwd in place of x; NULL: none */
     uint8_t* q_code;       /* [N, L, ceil(C / 32)] its exponents */
-    float* ws;             /* mtts_group_norm_workspace_floats(N, L, C, G) floats */
+    float* ws;             /* mtts_group_norm_workspace_floats floats (may be NULL where that is 0) */
     int N;
     int L;
     int C;
@@ -158,7 +158,7 @@ typedef struct GroupNormArgs {
     float* dbeta;
 } GroupNormArgs;
 
-long mtts_group_norm_workspace_floats(int N, int L, int C, int G);
+long mtts_group_norm_workspace_floats(const GroupNormArgs* args, int backward);      /* every other field as in the call; -1: bad arguments */
 int mtts_group_norm_act_fwd(const GroupNormArgs* args, void* stream);
 int mtts_group_norm_act_bwd(const GroupNormArgs* args, void* stream);
 

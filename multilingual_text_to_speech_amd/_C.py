@@ -112,6 +112,12 @@ def lib():
         _lib.mtts_gemm_planes_count.restype = ctypes.c_long
         _lib.mtts_group_norm_workspace_floats.restype = ctypes.c_long
         _lib.mtts_conv_weight_grad8_workspace_floats.restype = ctypes.c_long
+        _lib.mtts_group_norm_workspace_floats.argtypes = [ctypes.c_void_p, ctypes.c_int]
+        _lib.mtts_conv_weight_grad8_workspace_floats.argtypes = [ctypes.c_void_p]
+        for name in ('mtts_group_norm_act_fwd', 'mtts_group_norm_act_bwd', 'mtts_conv_weight_grad8'):
+            getattr(_lib, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        _lib.mtts_checkpoint8_pack.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int] * 4 + [ctypes.c_void_p]
+        _lib.mtts_checkpoint8_unpack.argtypes = [ctypes.c_void_p] * 3 + [ctypes.c_long, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
         _lib.mtts_set_workspace.argtypes = [ctypes.c_void_p, ctypes.c_size_t]
         _lib.mtts_set_stream_workspace.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t]
     return _lib
@@ -154,6 +160,13 @@ def ptr(t):
 def stream_ptr():
     import torch
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def stream_of(device):
+    """The current stream of a tensor's device as a plain number.  (torch.cuda.current_stream() builds a Stream object: 3 us a call.)"""
+    import torch
+    raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+    return raw(device.index) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def require_gpu(*tensors):

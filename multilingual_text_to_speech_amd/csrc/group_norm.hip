@@ -744,26 +744,25 @@ static int gn_check(const GroupNormArgs& p, const char* what) {
     MTTS_REQUIRE(p.C % p.G == 0, "%s: %d channels are not a multiple of %d groups", what, p.C, p.G);
     MTTS_REQUIRE(p.dtype == MTTS_F32 || p.dtype == MTTS_BF16, "%s: dtype %d is neither MTTS_F32 nor MTTS_BF16", what, p.dtype);
     MTTS_REQUIRE(p.act >= MTTS_ACT_NONE && p.act <= MTTS_ACT_SILU, "%s: unknown activation %d", what, p.act);
-    MTTS_REQUIRE(p.gamma && p.beta && p.mean && p.rstd && p.ws, "%s: missing tensor", what);
+    MTTS_REQUIRE(p.gamma && p.beta && p.mean && p.rstd, "%s: missing tensor", what);
     // a grid has fewer than 2^32 threads; strips are 32 channels wide at least, or the whole row
     MTTS_REQUIRE((long)p.N * cdiv(p.C, 32) * (p.G > cdiv(p.C, 32) ? 2 : 1) < (1L << 32) / 1024, "%s: %d samples x %d channels are too many for one call", what, p.N, p.C);
     MTTS_REQUIRE(p.C <= (1 << 24), "%s: %d channels are too many", what, p.C);
     return 0;
 }
 
-MTTS_API long mtts_group_norm_workspace_floats(int N, int L, int C, int G) {
-    if (N <= 0 || L <= 0 || C <= 0 || G <= 0 || C % G) return 0;
-    GroupNormArgs p;
-    memset(&p, 0, sizeof(p));
-    p.N = N; p.L = L; p.C = C; p.G = G;
-    long most = 0;
-    for (int i = 0; i < 8; ++i) {                // whatever type, addresses and direction the call will have
-        p.dtype = i & 1 ? MTTS_BF16 : MTTS_F32;
-        const GnGeo g = gn_plan(p, i & 2, i & 4).geo;
-        const long n = 2L * N * g.chunks * C + 3L * N * G * g.chunks * g.parts;
-        if (n > most) most = n;
-    }
-    return most;
+static bool gn_aligned(const GroupNormArgs& p, bool bwd) {
+    const int vec = p.dtype == MTTS_F32 ? 4 : 8;
+    return aligned_to(p.mask, vec) && aligned_to(p.q, vec) && (bwd ? (p.q || aligned_to(p.x, 16)) && aligned_to(p.dy, 16) && aligned_to(p.dx, 16) : aligned_to(p.x, 16) && aligned_to(p.y, 16));
+}
+
+// What the call with these arguments (all but ws filled in) needs.
+MTTS_API long mtts_group_norm_workspace_floats(const GroupNormArgs* args, int backward) {
+    const GroupNormArgs& p = *args;
+    if (gn_check(p, "mtts_group_norm_workspace_floats")) return -1;
+    const GnPlan k = gn_plan(p, gn_aligned(p, backward != 0), backward != 0);
+    const long sums = backward ? 2L * p.N * k.geo.chunks * p.C : 0;
+    return sums + (k.resident ? 0 : 3L * p.N * p.G * k.geo.chunks * k.geo.parts);
 }
 
 template <typename F> static int gn_attr(F fn, size_t lds) {
@@ -820,8 +819,8 @@ MTTS_API int mtts_group_norm_act_fwd(const GroupNormArgs* args, void* stream) {
     hipStream_t s = (hipStream_t)stream;
     MTTS_TRY(gn_check(p, "mtts_group_norm_act_fwd"));
     MTTS_REQUIRE(p.x && p.y && !p.q == !p.q_code, "mtts_group_norm_act_fwd: missing tensor");
-    const int vec = p.dtype == MTTS_F32 ? 4 : 8;
-    const GnPlan k = gn_plan(p, aligned_to(p.x, 16) && aligned_to(p.y, 16) && aligned_to(p.mask, vec) && aligned_to(p.q, vec), false);
+    const GnPlan k = gn_plan(p, gn_aligned(p, false), false);
+    MTTS_REQUIRE(p.ws || k.resident, "mtts_group_norm_act_fwd: missing workspace");
     int8_t* const q = p.q;
     if (!k.fuse) p.q = nullptr;                  // a pass of its own below
     if (p.dtype == MTTS_F32) {
@@ -847,8 +846,8 @@ MTTS_API int mtts_group_norm_act_bwd(const GroupNormArgs* args, void* stream) {
     hipStream_t s = (hipStream_t)stream;
     MTTS_TRY(gn_check(p, "mtts_group_norm_act_bwd"));
     MTTS_REQUIRE(p.dy && p.dx && (p.q ? p.q_code != nullptr : p.x != nullptr), "mtts_group_norm_act_bwd: missing tensor");
-    const int vec = p.dtype == MTTS_F32 ? 4 : 8;
-    const GnPlan k = gn_plan(p, (p.q || aligned_to(p.x, 16)) && aligned_to(p.dy, 16) && aligned_to(p.dx, 16) && aligned_to(p.mask, vec) && aligned_to(p.q, vec), true);
+    MTTS_REQUIRE(p.ws, "mtts_group_norm_act_bwd: missing workspace");
+    const GnPlan k = gn_plan(p, gn_aligned(p, true), true);
     if (p.dtype == MTTS_F32) {
         if (k.vec == 1) MTTS_TRY((gn_bwd_any<float, 1, false>(p, k, s)));
         else if (k.str) MTTS_TRY((gn_bwd_any<float, 4, true>(p, k, s)));

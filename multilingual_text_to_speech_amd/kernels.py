@@ -9,7 +9,7 @@ import os
 import torch
 
 from . import _C
-from ._C import check, lib, ptr, require_gpu, stream_ptr
+from ._C import check, lib, ptr, require_gpu, stream_of, stream_ptr
 
 ACT = {'identity': 0, 'relu': 1, 'tanh': 2, 'sigmoid': 3}
 
@@ -439,10 +439,14 @@ def _first_derivative_only(what):
         _refuse(what, 'there is no second derivative (create_graph=True)')
 
 
-def _same_device(what, device, **tensors):
-    for name, t in tensors.items():
+def _same_device(what, device, *tensors):
+    for t in tensors:
         if t is not None and t.device != device:
-            _refuse(what, f'{name} is on {t.device}, the input on {device}')
+            _refuse(what, f'the input is on {device}, another operand on {t.device}')
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 class _On:
@@ -470,7 +474,7 @@ def _check_lengths(what, lengths, N, L, device):
     if tuple(lengths.shape) != (N,) or lengths.dtype not in (torch.int32, torch.int64):
         _refuse(what, f'lengths is {lengths.dtype} {tuple(lengths.shape)}: int32 or int64 of shape ({N},) is expected')
     if lengths.is_cuda:
-        _same_device(what, device, lengths=lengths)
+        _same_device(what, device, lengths)
     elif N and (int(lengths.min()) < 0 or int(lengths.max()) > L):
         _refuse(what, f'lengths run from {int(lengths.min())} to {int(lengths.max())}: 0 to {L} is expected')
     return lengths
@@ -500,7 +504,7 @@ class Checkpoint8:
             _refuse('Checkpoint8', f'scales have shape {tuple(scales.shape)}: {want} is expected for values of shape {tuple(values.shape)}')
         if dtype not in _DTYPE:
             _refuse('Checkpoint8', f'dtype is {dtype}: float32 or bfloat16 is expected')
-        _same_device('Checkpoint8', values.device, scales=scales)
+        _same_device('Checkpoint8', values.device, scales)
         self.values, self.scales, self.dtype = values.contiguous(), scales.contiguous(), dtype
 
     @property
@@ -521,8 +525,8 @@ class Checkpoint8:
         if out.numel():
             C = out.shape[-1]
             with _On(out.device):
-                check(lib().mtts_checkpoint8_unpack(ptr(self.values), ptr(self.scales), ptr(out), ctypes.c_long(out.numel() // C), C,
-                                                    _DTYPE[dtype], stream_ptr()), 'checkpoint8_unpack')
+                check(lib().mtts_checkpoint8_unpack(self.values.data_ptr(), self.scales.data_ptr(), out.data_ptr(), out.numel() // C, C,
+                                                    _DTYPE[dtype], stream_of(out.device)), 'checkpoint8_unpack')
         return out
 
 
@@ -547,7 +551,7 @@ def checkpoint8(x, lengths=None):
         N, L = (x.shape[0], x.shape[1]) if lengths is not None else (1, x.numel() // C)
         with _On(x.device):
             lens = _device_lengths(what, lengths, x.device)
-            check(lib().mtts_checkpoint8_pack(ptr(x), ptr(lens), ptr(values), ptr(scales), N, L, C, _DTYPE[x.dtype], stream_ptr()), what)
+            check(lib().mtts_checkpoint8_pack(x.data_ptr(), _at(lens), values.data_ptr(), scales.data_ptr(), N, L, C, _DTYPE[x.dtype], stream_of(x.device)), what)
     return Checkpoint8(values, scales, x.dtype)
 
 
@@ -562,7 +566,7 @@ def conv1d_weight_grad8(held, dy, kernel, dilation=1, groups=1, packed=False):
         _refuse(what, f'kernel {kernel}, dilation {dilation}, groups {groups}: whole numbers of 1 and more are expected')
     if held.shape[:-1] != dy.shape[:-1] or dy.dim() < 1 or (kernel > 1 and dy.dim() != 3):
         _refuse(what, f'input {tuple(held.shape)} and gradient {tuple(dy.shape)} do not belong to one convolution of kernel {kernel}')
-    _same_device(what, dy.device, checkpoint=held.values)
+    _same_device(what, dy.device, held.values)
     I, O = held.shape[-1], dy.shape[-1]
     if I % groups or O % groups or not I or not O:
         _refuse(what, f'{I} x {O} channels are not a multiple of {groups} groups')
@@ -581,40 +585,50 @@ def conv1d_weight_grad8(held, dy, kernel, dilation=1, groups=1, packed=False):
         if n < 0:
             _refuse(what, lib().mtts_last_error().decode())
         ws = _f32(n, device=dy.device) if n else None
-        a.ws = ptr(ws)
-        check(lib().mtts_conv_weight_grad8(ctypes.byref(a), stream_ptr()), what)
+        a.ws = _at(ws)
+        check(lib().mtts_conv_weight_grad8(ctypes.byref(a), stream_of(dy.device)), what)
     return dw
 
 
 def _gn_fwd(x, gamma, beta, groups, lengths, mask, act, eps, mask_scale, checkpoint):
-    """y, mean, rstd, checkpoint values / scales (or None) of contiguous operands."""
+    """y, mean and rstd [2, N, G], checkpoint values / scales (or None) of contiguous operands."""
     N, L, C = x.shape
     dev = x.device
     y = torch.empty_like(x)
     stats = _f32(2, N, groups, device=dev)
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev) if checkpoint else None
-    code = torch.empty(N, L, -(-C // CHECKPOINT_BLOCK), dtype=torch.uint8, device=dev) if checkpoint else None
+    q = code = None
+    if checkpoint:
+        q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+        code = torch.empty(N, L, -(-C // CHECKPOINT_BLOCK), dtype=torch.uint8, device=dev)
     if x.numel():
-        ws = _f32(lib().mtts_group_norm_workspace_floats(N, L, C, groups), device=dev)
-        a = _C.GroupNormArgs(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), ptr(lengths), ptr(mask), y.data_ptr(), stats.data_ptr(),
-                             stats.data_ptr() + 4 * N * groups, ptr(q), ptr(code), ws.data_ptr(), N, L, C, groups, _DTYPE[x.dtype], act, eps, mask_scale)
-        check(lib().mtts_group_norm_act_fwd(ctypes.byref(a), stream_ptr()), 'group_norm_act_fwd')
+        at = stats.data_ptr()
+        a = _C.GroupNormArgs(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _at(lengths), _at(mask), y.data_ptr(), at, at + 4 * N * groups,
+                             _at(q), _at(code), None, N, L, C, groups, _DTYPE[x.dtype], act, eps, mask_scale)
+        _gn_launch('mtts_group_norm_act_fwd', a, 0, dev)
     return y, stats, q, code
+
+
+def _gn_launch(entry, a, backward, device):
+    at = ctypes.addressof(a)
+    n = lib().mtts_group_norm_workspace_floats(at, backward)
+    if n < 0:
+        _refuse(entry, lib().mtts_last_error().decode())
+    ws = _f32(n, device=device) if n else None
+    a.ws = _at(ws)
+    check(getattr(lib(), entry)(at, stream_of(device)), entry)
 
 
 def _gn_bwd(x, q, code, gamma, beta, stats, lengths, mask, dy, groups, act, eps, mask_scale):
     """dx, dgamma, dbeta; x may be None where the checkpoint (q, code) holds it."""
     N, L, C = dy.shape
-    dev = dy.device
     dx = torch.empty_like(dy)
     if not dy.numel():
         return dx, torch.zeros_like(gamma), torch.zeros_like(beta)
     dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
-    ws = _f32(lib().mtts_group_norm_workspace_floats(N, L, C, groups), device=dev)
-    a = _C.GroupNormArgs(ptr(x), gamma.data_ptr(), beta.data_ptr(), ptr(lengths), ptr(mask), None, stats.data_ptr(),
-                         stats.data_ptr() + 4 * N * groups, ptr(q), ptr(code), ws.data_ptr(), N, L, C, groups, _DTYPE[dy.dtype], act, eps, mask_scale,
-                         dy.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr())
-    check(lib().mtts_group_norm_act_bwd(ctypes.byref(a), stream_ptr()), 'group_norm_act_bwd')
+    at = stats.data_ptr()
+    a = _C.GroupNormArgs(_at(x), gamma.data_ptr(), beta.data_ptr(), _at(lengths), _at(mask), None, at, at + 4 * N * groups, _at(q), _at(code), None,
+                         N, L, C, groups, _DTYPE[dy.dtype], act, eps, mask_scale, dy.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr())
+    _gn_launch('mtts_group_norm_act_bwd', a, 1, dy.device)
     return dx, dgamma, dbeta
 
 
@@ -654,7 +668,7 @@ def _gn_check(what, shape, device, gamma, beta, groups, lengths, mask, act):
         if mask.dtype not in (torch.uint8, torch.bool) or tuple(mask.shape) != (N, L, C):
             _refuse(what, f'mask is {mask.dtype} {tuple(mask.shape)}: uint8 keep flags of shape {(N, L, C)} are expected')
         mask = mask.contiguous().view(torch.uint8)
-    _same_device(what, device, gamma=gamma, beta=beta, mask=mask)
+    _same_device(what, device, gamma, beta, mask)
     return gamma.contiguous(), beta.contiguous(), _check_lengths(what, lengths, N, L, device), mask
 
 
@@ -725,7 +739,7 @@ def conv_gn_act(x, weight, gamma, beta, lengths=None, mask=None, *, kernel, norm
         _refuse(what, f'x {x.dtype} {tuple(x.shape)}, weight {weight.dtype} {tuple(weight.shape)}: float32 [N, L, I] and [O, I / groups, kernel] are expected')
     if min(kernel, dilation, groups) < 1 or not x.numel() or tuple(weight.shape[1:]) != (x.shape[2] // groups, kernel) or x.shape[2] % groups or weight.shape[0] % groups:
         _refuse(what, f'input {tuple(x.shape)} and weight {tuple(weight.shape)} do not belong to one convolution of kernel {kernel} with {groups} groups')
-    _same_device(what, x.device, weight=weight)
+    _same_device(what, x.device, weight)
     gamma, beta, lengths, mask = _gn_check(what, (x.shape[0], x.shape[1], weight.shape[0]), x.device, gamma, beta, norm_groups, lengths, mask, act)
     require_gpu(x)
     learns = torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, gamma, beta))

@@ -104,6 +104,12 @@ def test_entry_points_refuse_before_they_launch(library):
     assert library.mtts_group_norm_act_fwd(ctypes.byref(a), None) and 'missing tensor' in err()
     a.N, a.q = 0, None
     assert library.mtts_group_norm_act_fwd(ctypes.byref(a), None) and 'empty' in err()
+    assert library.mtts_group_norm_workspace_floats(ctypes.byref(a), 0) == -1
+    a.N, a.L, a.ws = 2, 100000, None                                # too long for one workgroup: a workspace is needed
+    assert library.mtts_group_norm_workspace_floats(ctypes.byref(a), 0) > 0
+    assert library.mtts_group_norm_act_fwd(ctypes.byref(a), None) and 'workspace' in err()
+    a.dy = a.dx = 4096
+    assert library.mtts_group_norm_act_bwd(ctypes.byref(a), None) and 'workspace' in err()
     a.N, a.C, a.G = 1 << 30, 64, 1
     assert library.mtts_group_norm_act_fwd(ctypes.byref(a), None) and 'too many' in err()
     assert library.mtts_checkpoint8_pack(p, None, p, None, 1, 1, 1, 0, None) and 'missing tensor' in err()
@@ -179,3 +185,13 @@ def test_round_trip_definition():
     q, code, v = R.round_trip(y)
     assert ((v - y).abs() <= torch.pow(2.0, code.double() - 128).repeat_interleave(32, -1)[:, :77]).all()
     assert torch.equal(v.bfloat16().double(), v)                                         # exact in bfloat16
+
+
+def test_entry_points_take_whole_addresses(library):
+    """Addresses are passed as Python numbers: every entry that takes one has to say that it is a pointer (a bare number is a C int)."""
+    for name in ('mtts_group_norm_workspace_floats', 'mtts_group_norm_act_fwd', 'mtts_group_norm_act_bwd', 'mtts_conv_weight_grad8',
+                 'mtts_conv_weight_grad8_workspace_floats', 'mtts_checkpoint8_pack', 'mtts_checkpoint8_unpack'):
+        f = getattr(library, name)
+        assert f.argtypes is not None and f.argtypes[0] is ctypes.c_void_p, name
+    a = _C.GroupNormArgs(gamma=4096, beta=4096, mean=4096, rstd=4096, x=4096, y=4096, N=2, L=3, C=8, G=2)
+    assert library.mtts_group_norm_workspace_floats(ctypes.addressof(a), 0) == 0
