@@ -35,23 +35,24 @@ template <int ACT> __device__ __forceinline__ float gn_act(float z) {
     if constexpr (ACT == MTTS_ACT_SILU) return z * gn_sigmoid(z);
     return z;
 }
-// d * act'(z); relu: 0 at z = 0, as the framework's other blocks
-template <int ACT> __device__ __forceinline__ float gn_act_slope(float z, float d) {
-    if constexpr (ACT == MTTS_ACT_RELU) return z > 0.f ? d : 0.f;
-    if constexpr (ACT == MTTS_ACT_TANH) {      // 1 - tanh^2 = 4 e / (1 + e)^2: no cancellation in the tails
-        const float e = __expf(-2.f * fabsf(z)), r = __builtin_amdgcn_rcpf(1.f + e);
-        return d * (4.f * e * r * r);
+// act'(z) of every activation from one exponential, without a branch (rows in registers, see GN_ROW_DONE): with e = exp(-k |z|),
+// w = e / (1 + e)^2 = p (1 - p) and p = sigmoid(k z):  c0 + c1 w + c2 p + c3 z w, nothing at or below `floor`.  tanh: 1 - tanh^2 = 4 w at
+// k = 2, no cancellation in the tails; silu: p + z p (1 - p); relu: 1 above zero, as the framework's other blocks.
+struct GnSlope {
+    float k, c0, c1, c2, c3, floor;
+    __device__ __forceinline__ explicit GnSlope(int act) {
+        k = act == MTTS_ACT_TANH ? -2.f : -1.f;
+        c0 = act == MTTS_ACT_NONE || act == MTTS_ACT_RELU ? 1.f : 0.f;
+        c1 = act == MTTS_ACT_TANH ? 4.f : act == MTTS_ACT_SIGMOID ? 1.f : 0.f;
+        c2 = c3 = act == MTTS_ACT_SILU ? 1.f : 0.f;
+        floor = act == MTTS_ACT_RELU ? 0.f : -__builtin_inff();
     }
-    if constexpr (ACT == MTTS_ACT_SIGMOID) {
-        const float e = __expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.f + e);
-        return d * (e * r * r);
+    __device__ __forceinline__ float operator()(float z) const {
+        const float e = __expf(k * fabsf(z)), r = __builtin_amdgcn_rcpf(1.f + e), w = e * r * r, p = z < 0.f ? e * r : r;
+        const float s = c0 + w * (c1 + c3 * fminf(fmaxf(z, -1e30f), 1e30f)) + c2 * p;
+        return z <= floor ? 0.f : s;
     }
-    if constexpr (ACT == MTTS_ACT_SILU) {
-        const float g = gn_sigmoid(z);
-        return d * (g * (1.f + z * (1.f - g)));
-    }
-    return d;
-}
+};
 // body(integral constant of the activation): one uniform branch around a whole loop over rows
 template <int A> struct GnAct { static constexpr int value = A; };
 template <typename F> __device__ __forceinline__ void gn_by_act(int act, F body) {
@@ -74,7 +75,10 @@ __device__ __forceinline__ int gn_length(const GroupNormArgs& p, int n) { return
 struct GnTile { int n, chunk, strip, g0, c0, c1, c, tx, ty, TY, len; bool on; };
 template <int VEC> __device__ __forceinline__ GnTile gn_tile(const GroupNormArgs& p, const GnGeo& k) {
     GnTile t;
-    unsigned b = blockIdx.x;
+    // workgroups go to the eight XCDs in turn; each XCD gets a contiguous run of strips, so that neighbouring strips (which share lines of
+    // the checkpoint and pages of the rest) meet in one L2: backward at 64 x 600 x 512, fp32 60.5 -> 55 us
+    const unsigned per = gridDim.x >> 3, rem = gridDim.x & 7, xcd = blockIdx.x & 7;
+    unsigned b = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
     t.strip = b % k.strips; b /= k.strips;
     t.chunk = b % k.chunks; t.n = b / k.chunks;
     const int Cg = p.C / p.G;
@@ -127,6 +131,9 @@ template <int TAG = -1, typename V> __device__ __forceinline__ void gn_forget(V&
     }
 }
 
+// A running sum is taken here: its additions must not sink, with all their terms, to the place where the sum is used.
+__device__ __forceinline__ void gn_pin(float& v) { asm volatile("" : "+v"(v)); }
+
 // Element offsets of a thread's rows in its sample, one after the other; a thread without a vector stays at GN_OUT.
 struct GnWalk {
     unsigned at, step; bool on;
@@ -142,7 +149,7 @@ __device__ __forceinline__ float gn_drop(const GroupNormArgs& p, unsigned keep, 
 
 // STR: a vector may straddle groups (statistics per channel of the vector, else one set per thread)
 template <typename T, int VEC, int R, bool STR>
-__global__ void __launch_bounds__(R > 8 ? 512 : 1024) gn_fwd_kernel(GroupNormArgs p, GnGeo k) {
+__global__ void __launch_bounds__(R > 12 ? 512 : 1024) gn_fwd_kernel(GroupNormArgs p, GnGeo k) {
     constexpr int SZ = sizeof(T), K = STR ? VEC : 1;
     extern __shared__ float lds[];
     const GnTile t = gn_tile<VEC>(p, k);
@@ -181,6 +188,7 @@ __global__ void __launch_bounds__(R > 8 ? 512 : 1024) gn_fwd_kernel(GroupNormArg
 #pragma unroll
             for (int q = 0; q < VEC / K; ++q) v += x[i].at(STR ? j : q);
             s += v;
+            gn_pin(s);
         }
         if (t.ty < t.TY) red[slot[j]] = s;
     }
@@ -203,6 +211,7 @@ __global__ void __launch_bounds__(R > 8 ? 512 : 1024) gn_fwd_kernel(GroupNormArg
                 const float d = i < valid ? x[i].at(STR ? j : q) - mean[j] : 0.f;
                 s += d; s2 += d * d;
             }
+            gn_pin(s); gn_pin(s2);
         }
         if (t.ty < t.TY) { red[slot[j]] = s; red[k.NG * E + slot[j]] = s2; }
     }
@@ -237,7 +246,7 @@ __global__ void __launch_bounds__(R > 8 ? 512 : 1024) gn_fwd_kernel(GroupNormArg
                 const float z = gn_act<act.value>((v.at(j) - mean[STR ? j : 0]) * rstd[STR ? j : 0] * gamma[j] + beta[j]);
                 f[j] = i < valid ? gn_drop(p, keep[i].get(j), z) : 0.f;
             }
-            store_vec(ry, w.bytes(SZ), f);
+            stream_vec(ry, w.bytes(SZ), f);
         }
     });
     if (!p.q) return;
@@ -264,13 +273,13 @@ __global__ void __launch_bounds__(R > 8 ? 512 : 1024) gn_fwd_kernel(GroupNormArg
 }
 
 // xhat and dz of one row vector
-template <int ACT, typename T, int VEC, int K> __device__ __forceinline__ void gn_dz(const GroupNormArgs& p, const float (&mean)[K], const float (&rstd)[K], const float (&gamma)[VEC], const float (&beta)[VEC],
-                                                                                     const Bytes<VEC>& keep, const Raw<T, VEC>& dy, const float (&x)[VEC], float (&xhat)[VEC], float (&dz)[VEC]) {
+template <typename T, int VEC, int K> __device__ __forceinline__ void gn_dz(const GroupNormArgs& p, const GnSlope& slope, const float (&mean)[K], const float (&rstd)[K], const float (&gamma)[VEC], const float (&beta)[VEC],
+                                                                           const Bytes<VEC>& keep, const Raw<T, VEC>& dy, const float (&x)[VEC], float (&xhat)[VEC], float (&dz)[VEC]) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         const float u = (x[j] - mean[K > 1 ? j : 0]) * rstd[K > 1 ? j : 0];
         xhat[j] = u;
-        dz[j] = gn_act_slope<ACT>(u * gamma[j] + beta[j], gn_drop(p, keep.get(j), dy.at(j)));
+        dz[j] = gn_drop(p, keep.get(j), dy.at(j)) * slope(u * gamma[j] + beta[j]);
     }
 }
 
@@ -331,25 +340,21 @@ __global__ void __launch_bounds__(512) gn_bwd_kernel(GroupNormArgs p, GnGeo k) {
     float dz[R][VEC], s1[VEC], s2[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) s1[j] = s2[j] = 0.f;
-    gn_by_act(p.act, [&](auto act) __attribute__((always_inline)) {
+    const GnSlope slope(p.act);
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            GN_ROW_DONE;
-            GnX<T, VEC, CK> xi = x[i];
-            Raw<T, VEC> di = dy[i];
-            gn_forget<act.value>(xi.w.w);
-            gn_forget<act.value>(di.w);
-            float f[VEC], xh[VEC], d[VEC];
-            xi.get(f);
-            gn_dz<act.value, T, VEC, K>(p, mean, rstd, gamma, beta, keep[i], di, f, xh, d);
+    for (int i = 0; i < R; ++i) {
+        GN_ROW_DONE;
+        float f[VEC], xh[VEC], d[VEC];
+        x[i].get(f);
+        gn_dz<T, VEC, K>(p, slope, mean, rstd, gamma, beta, keep[i], dy[i], f, xh, d);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float v = i < valid ? d[j] : 0.f;
-                dz[i][j] = v;
-                s1[j] += v; s2[j] += i < valid ? v * xh[j] : 0.f;
-            }
+        for (int j = 0; j < VEC; ++j) {
+            const float v = i < valid ? d[j] : 0.f;
+            dz[i][j] = v;
+            s1[j] += v; s2[j] += i < valid ? v * xh[j] : 0.f;
+            gn_pin(s1[j]); gn_pin(s2[j]);
         }
-    });
+    }
     if (t.ty < t.TY) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) { red[j * TS + threadIdx.x] = s1[j]; red[(VEC + j) * TS + threadIdx.x] = s2[j]; }
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(512) gn_bwd_kernel(GroupNormArgs p, GnGeo k) {
             const float xh = (f[j] - mean[u]) * rstd[u];
             dx[j] = i < valid ? rstd[u] * (gamma[j] * dz[i][j] - m1[u] - xh * m2[u]) : 0.f;
         }
-        store_vec(ro, w.bytes(SZ), dx);
+        stream_vec(ro, w.bytes(SZ), dx);
     }
 }
 
@@ -528,7 +533,7 @@ __global__ void __launch_bounds__(GN_T) gn_apply_kernel(GroupNormArgs p, GnGeo k
                     const float z = gn_act<act.value>((v[u].at(j) - mean[STR ? j : 0]) * rstd[STR ? j : 0] * gamma[j] + beta[j]);
                     f[j] = rr < rv ? gn_drop(p, keep[u].get(j), z) : 0.f;
                 }
-                store_vec((T*)p.y + base + (long)rr * p.C, f);
+                stream_vec((T*)p.y + base + (long)rr * p.C, f);
             }
         }
     });
@@ -573,21 +578,20 @@ __global__ void __launch_bounds__(GN_T) gn_bwd_sums_kernel(GroupNormArgs p, GnGe
     if (t.on) {
         GnCol<VEC, STR ? VEC : 1> col;
         col.load(p, t);
-        gn_by_act(p.act, [&](auto act) __attribute__((always_inline)) {
-            for (int r = r0 + t.ty; r < rv; r += GN_U * t.TY) {
-                GnRows<T, VEC, CK> w;
-                w.load(p, (long)t.n * p.L, r, t.TY, rv, t.c);
+        const GnSlope slope(p.act);
+        for (int r = r0 + t.ty; r < rv; r += GN_U * t.TY) {
+            GnRows<T, VEC, CK> w;
+            w.load(p, (long)t.n * p.L, r, t.TY, rv, t.c);
 #pragma unroll
-                for (int u = 0; u < GN_U; ++u) {
-                    if (r + u * t.TY >= rv) break;
-                    float f[VEC], xh[VEC], dz[VEC];
-                    w.x[u].get(f);
-                    gn_dz<act.value, T, VEC, STR ? VEC : 1>(p, col.mean, col.rstd, col.gamma, col.beta, w.keep[u], w.dy[u], f, xh, dz);
+            for (int u = 0; u < GN_U; ++u) {
+                if (r + u * t.TY >= rv) break;
+                float f[VEC], xh[VEC], dz[VEC];
+                w.x[u].get(f);
+                gn_dz<T, VEC, STR ? VEC : 1>(p, slope, col.mean, col.rstd, col.gamma, col.beta, w.keep[u], w.dy[u], f, xh, dz);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) { s1[j] += dz[j]; s2[j] += dz[j] * xh[j]; }
-                }
+                for (int j = 0; j < VEC; ++j) { s1[j] += dz[j]; s2[j] += dz[j] * xh[j]; }
             }
-        });
+        }
     }
     if (t.ty < t.TY) {
 #pragma unroll
@@ -634,27 +638,26 @@ __global__ void __launch_bounds__(GN_T) gn_bwd_apply_kernel(GroupNormArgs p, GnG
     for (int j = 0; j < K; ++j) { const int g = k.parts > 1 ? 0 : (t.tx * VEC + j) / Cg; m1[j] = mid[2 * g]; m2[j] = mid[2 * g + 1]; }
     const int per = (p.L + k.chunks - 1) / k.chunks, r0 = t.chunk * per, r1 = min(p.L, r0 + per), rv = min(r1, t.len);
     const long base = (long)t.n * p.L * p.C + t.c;
-    gn_by_act(p.act, [&](auto act) __attribute__((always_inline)) {
-        for (int r = r0 + t.ty; r < r1; r += GN_U * t.TY) {
-            GnRows<T, VEC, CK> w;
-            if (r < rv) w.load(p, (long)t.n * p.L, r, t.TY, rv, t.c);
+    const GnSlope slope(p.act);
+    for (int r = r0 + t.ty; r < r1; r += GN_U * t.TY) {
+        GnRows<T, VEC, CK> w;
+        if (r < rv) w.load(p, (long)t.n * p.L, r, t.TY, rv, t.c);
 #pragma unroll
-            for (int u = 0; u < GN_U; ++u) {
-                const int rr = r + u * t.TY;
-                if (rr >= r1) break;
-                float f[VEC], xh[VEC], dz[VEC], dx[VEC];
+        for (int u = 0; u < GN_U; ++u) {
+            const int rr = r + u * t.TY;
+            if (rr >= r1) break;
+            float f[VEC], xh[VEC], dz[VEC], dx[VEC];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) dx[j] = 0.f;
-                if (rr < rv) {
-                    w.x[u].get(f);
-                    gn_dz<act.value, T, VEC, K>(p, col.mean, col.rstd, col.gamma, col.beta, w.keep[u], w.dy[u], f, xh, dz);
+            for (int j = 0; j < VEC; ++j) dx[j] = 0.f;
+            if (rr < rv) {
+                w.x[u].get(f);
+                gn_dz<T, VEC, K>(p, slope, col.mean, col.rstd, col.gamma, col.beta, w.keep[u], w.dy[u], f, xh, dz);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) { const int v = STR ? j : 0; dx[j] = col.rstd[v] * (col.gamma[j] * dz[j] - m1[v] - xh[j] * m2[v]); }
-                }
-                store_vec((T*)p.dx + base + (long)rr * p.C, dx);
+                for (int j = 0; j < VEC; ++j) { const int v = STR ? j : 0; dx[j] = col.rstd[v] * (col.gamma[j] * dz[j] - m1[v] - xh[j] * m2[v]); }
             }
+            stream_vec((T*)p.dx + base + (long)rr * p.C, dx);
         }
-    });
+    }
 }
 
 // dgamma, dbeta: sums over the rows of ws[2][rows][C] in row order.  grid ceil(C / 64), block 64 x 16
@@ -696,13 +699,16 @@ static GnPlan gn_plan(const GroupNormArgs& p, bool wide, bool bwd) {
     wide = wide && p.C % full == 0 && (gn_lcm(Cg, full) <= GN_T * full || Cg % full == 0);
     k.vec = wide ? full : 1;
     k.str = Cg % k.vec != 0;
-    // a strip: whole groups and vectors, at least a 128-byte line of a row, whole checkpoint blocks where that is not much wider
-    const int unit = gn_lcm(Cg, k.vec), line = 128 / sz, blocks = gn_lcm(unit, CK_BLOCK);
+    // A strip: whole groups and vectors, whole checkpoint blocks where that is not much wider, and at least a 128-byte line of a row (the
+    // bf16 backward: 64 bytes and two workgroups to a CU, 41 -> 35 us at 64 x 600 x 512).  The same with and without a checkpoint, so
+    // that y does not depend on it.
+    const int unit = gn_lcm(Cg, k.vec), line = bwd || sz == 4 ? 32 : 64, blocks = gn_lcm(unit, CK_BLOCK);
     int W = (blocks <= 2 * line || blocks <= 2 * unit) ? blocks : unit;
     W *= cdiv(line, W);
     if (W > p.C) W = p.C;
-    // resident: one workgroup, R vectors per thread, as few threads as keep R small; offsets in a sample below 2^31 bytes.
-    // Register budgets: 1024 threads hold 8 vectors of the forward each, 512 threads 16; the backward's 512 threads 16 (bf16: 12).
+    // resident: one workgroup, R vectors per thread; offsets in a sample below 2^31 bytes.  Small workgroups with few vectors each where
+    // that holds the strip (64 x 117 rows of bf16: 128 threads of 8 vectors 11.8 us, 256 of 4 9.2 us), then up to 12 vectors for 256
+    // threads (300 rows, backward: 512 threads of 8 33 us, 256 of 10 23 us), 16 for 512, 12 for the forward's 1024.
     g.parts = 1; g.chunks = 1;
     g.TX = cdiv(W, k.vec);
     k.resident = false;
@@ -710,10 +716,10 @@ static GnPlan gn_plan(const GroupNormArgs& p, bool wide, bool bwd) {
         for (int T = 64; T <= (bwd ? 512 : 1024) && !k.resident; T *= 2) {
             if (T < g.TX) continue;
             const int r = cdiv(p.L, T / g.TX);
-            const int most = T < 512 ? 8 : T == 1024 ? 8 : bwd && sz == 2 ? 12 : 16;
+            const int most = T < 256 ? 4 : T == 512 ? 16 : 12;
             if (r > most) continue;
             k.threads = T;
-            k.R = r <= 1 ? 1 : r <= 4 ? 4 : r <= 8 ? 8 : r <= 12 ? 12 : 16;
+            k.R = r <= 1 ? 1 : r <= 4 ? 4 : r <= 8 ? 8 : r <= 10 ? 10 : r <= 12 ? 12 : 16;
             k.resident = ((long)(T / g.TX) * k.R + 1) * p.C * sz < (1L << 32);      // offsets of rows behind the last do not wrap
         }
     if (!k.resident) {
@@ -789,6 +795,7 @@ template <typename T, int VEC, bool STR> static int gn_fwd_pick(const GroupNormA
             case 1: return gn_fwd_go<T, VEC, 1, STR>(p, k, s);
             case 4: return gn_fwd_go<T, VEC, 4, STR>(p, k, s);
             case 8: return gn_fwd_go<T, VEC, 8, STR>(p, k, s);
+            case 10: return gn_fwd_go<T, VEC, 10, STR>(p, k, s);
             case 12: return gn_fwd_go<T, VEC, 12, STR>(p, k, s);
             default: return gn_fwd_go<T, VEC, 16, STR>(p, k, s);
         }
@@ -804,8 +811,9 @@ template <typename T, int VEC, bool STR, bool CK> static int gn_bwd_pick(const G
             case 1: return gn_bwd_go<T, VEC, 1, STR, CK>(p, k, s);
             case 4: return gn_bwd_go<T, VEC, 4, STR, CK>(p, k, s);
             case 8: return gn_bwd_go<T, VEC, 8, STR, CK>(p, k, s);
+            case 10: return gn_bwd_go<T, VEC, 10, STR, CK>(p, k, s);
             case 12: return gn_bwd_go<T, VEC, 12, STR, CK>(p, k, s);
-            default: if constexpr (sizeof(T) == 4) return gn_bwd_go<T, VEC, 16, STR, CK>(p, k, s);
+            default: return gn_bwd_go<T, VEC, 16, STR, CK>(p, k, s);
         }
     }
     float* const gs = p.ws + 2L * p.N * k.geo.chunks * p.C;

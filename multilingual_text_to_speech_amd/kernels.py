@@ -425,6 +425,9 @@ _DTYPE = {torch.float32: 0, torch.bfloat16: 1}
 GN_ACT = {**ACT, 'silu': 4}
 
 
+_MOST_ROWS = 0x7fff0000                    # row numbers are 32-bit
+
+
 def _refuse(what, why):
     raise _C.MttsError(f'{what}: {why}')
 
@@ -542,6 +545,8 @@ def checkpoint8(x, lengths=None):
         _refuse(what, f'x has shape {tuple(x.shape)}: at least one channel is expected')
     if lengths is not None:
         lengths = _check_lengths(what, lengths, x.shape[0], x.shape[1], x.device)
+    if x.numel() // x.shape[-1] > _MOST_ROWS:
+        _refuse(what, f'{x.numel() // x.shape[-1]} rows are too many for one call')
     require_gpu(x)
     x = x.detach().contiguous()
     C = x.shape[-1]
@@ -570,6 +575,8 @@ def conv1d_weight_grad8(held, dy, kernel, dilation=1, groups=1, packed=False):
     I, O = held.shape[-1], dy.shape[-1]
     if I % groups or O % groups or not I or not O:
         _refuse(what, f'{I} x {O} channels are not a multiple of {groups} groups')
+    if dy.numel() // O > _MOST_ROWS:
+        _refuse(what, f'{dy.numel() // O} rows are too many for one call')
     require_gpu(held.values, dy)
     shape = (O, kernel, I // groups) if packed else (O, I // groups, kernel)
     rows = dy.numel() // O

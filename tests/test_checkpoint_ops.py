@@ -55,6 +55,9 @@ def test_checkpoint_refusals():
     refused('lengths need', K.checkpoint8, x[0], [1, 1])
     refused('lengths run', K.checkpoint8, x, [1, 5])
     refused('one channel', K.checkpoint8, torch.zeros(3, 0))
+    refused('too many', K.checkpoint8, torch.zeros(1, 1).expand(2 ** 31, 1))
+    refused('too many', K.conv1d_weight_grad8, K.Checkpoint8(torch.empty(2 ** 31, 1, dtype=torch.int8, device='meta'), torch.empty(2 ** 31, 1, dtype=torch.uint8, device='meta')),
+            torch.empty(2 ** 31, 1, device='meta'), 1)
     refused('int8', K.Checkpoint8, v.to(torch.uint8), s)
     refused('int8', K.Checkpoint8, v, s.to(torch.int8))
     refused('shape', K.Checkpoint8, v, s[..., :1])
