@@ -8,9 +8,10 @@
 // the leading eight bits of what is left (an exact split, 24 bits), against six where both operands are fp32.  fp32 accumulation.
 // A bf16 gradient, and an fp32 one in bf16 mode (rounded to nearest even), takes one term.
 //
-// What bounds it: the matrix pipes.  At 38400 rows, 512 -> 512 channels, kernel 5 (100.7 GFLOP, three terms) the whole call takes 248 us,
-// 1220 TFLOP/s of bf16 products where a plain bf16 library product of 8192^3 reaches 1330 on the same card; with a bf16 gradient 163 us.
-// At 7680 rows, bf16 (20 GFLOP) 48 us: a third of that is the partial tiles' way through memory (63 MB out and in at twelve splits).
+// What bounds it: the matrix pipes.  At 38400 rows, 512 -> 512 channels, kernel 5 (100.7 GFLOP, three terms) the whole call takes 243 us,
+// 1240 TFLOP/s of bf16 products where a plain bf16 library product of 8192^3 reaches 1330 on the same card.  One term (bf16 gradients):
+// 134 us, LDS traffic beside the matrix pipes.  At 7680 rows, bf16 (20 GFLOP) 46 us: half of that is the partial tiles' way through
+// memory (63 MB out and in at twelve splits).
 //
 // Tile TM x TN x 32 rows per workgroup, v_mfma_f32_32x32x16_bf16.  A thread takes 8 rows x 4 columns: the transposition happens in
 // registers, and 8 rows of one column are the 16 bytes that a lane feeds to the matrix instruction.  LDS holds these 16-byte units in
@@ -174,81 +175,94 @@ __global__ void __launch_bounds__(256) wgrad8_edge_kernel(Wgrad8Args p, int spli
     wg_store<2, 2>(p, splits, w.split, w.g, m0 + wm, n0 + wn, lane, acc);
 }
 
-// The pipelined form.  Two LDS stages; while the matrix instructions of step k run, the piece of step
-// k + 1 (its loads were issued a step earlier) is split and stored to the other stage and the loads of step k + 2 are issued: one
-// barrier a step.  The first TM threads stage dy, the other TN threads x, each half of the waves runs its own copy of the loop.
+// The pipelined form.  Two LDS stages: while the matrix instructions of step k run, the piece of step k + 1 is split and stored to the
+// other stage and the next loads are under way; one barrier a step.  The first TM threads stage dy, the other TN threads x, each half of the waves runs its own copy of the loop.
 // Loads go through buffer descriptors of the split's rows, which return zero behind the end; a row outside its sample is sent there.
 // ODD: quads of x or of a bf16 dy may start at any byte; the aligned words around them are loaded and shifted together.
-template <typename T, int TERMS, int TM, int TN, int WM, int WN, bool ODD>
-__global__ void __launch_bounds__(TM + TN) wgrad8_kernel(Wgrad8Args p, int splits, int tiles_m, int tiles_n, int steps_per) {
+template <int S> struct WgSet { static constexpr int value = S; };
+
+// KP: 32-row blocks of a step; each has waves of its own over the whole tile, whose accumulators are added at the end (through LDS).
+template <typename T, int TERMS, int TM, int TN, int WM, int WN, int KP, bool ODD>
+__global__ void __launch_bounds__((TM + TN) * KP) wgrad8_kernel(Wgrad8Args p, int splits, int tiles_m, int tiles_n, int steps_per) {
     static_assert((TM / WM) * (TN / WN) * 64 == TM + TN && TM % 64 == 0, "one 8 x 4 piece of an operand tile per thread, whole waves to each operand");
-    constexpr int FM = WM / 32, FN = WN / 32, PLANE = TM * 4, STAGE = TERMS * PLANE + TN * 4;
-    extern __shared__ u32x4 lds[];           // [2][STAGE]
+    constexpr int FM = WM / 32, FN = WN / 32, PLANE = TM * 4, BLOCK = TERMS * PLANE + TN * 4, STAGE = KP * BLOCK, BK = WG_BK * KP, SETS = TERMS == 1 || TM == 128 ? 2 : 1, WAVES = (TM / WM) * (TN / WN);
+    extern __shared__ u32x4 lds[];           // [2][KP][BLOCK]
     const int Og = p.O / p.groups, nb = (p.I + CK_BLOCK - 1) / CK_BLOCK;
     const WgAt w = wg_at(tiles_m, tiles_n, p.groups, gridDim.x);
     const int m0 = w.tm * TM, n0 = w.tn * TN, pad = (p.kernel - 1) * p.dilation / 2;
     const long R = (long)p.N * p.L, k_begin = (long)w.split * steps_per * WG_BK, k_end = min(R, k_begin + (long)steps_per * WG_BK);
-    const int steps = (int)((k_end - k_begin + WG_BK - 1) / WG_BK);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = (wave / (TN / WN)) * WM, wn = (wave % (TN / WN)) * WN;
+    const int steps = (int)((k_end - k_begin + BK - 1) / BK);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kp = wave / WAVES;
+    const int wm = (wave % WAVES / (TN / WN)) * WM, wn = (wave % (TN / WN)) * WN;
     f32x16 acc[FM][FN];
     wg_clear(acc);
 
+    // load(k, S): the rows of step k into register set S; put(S, stage).  With two sets the loads have a step and a half to arrive: a bf16
+    // step of 256 x 256 x 32 is half a microsecond of matrix instructions, less than the way to memory.
     auto loop = [&](auto load, auto put) {
-        load(0);
-        put(lds);
+        load(WgSet<0>());
+        put(WgSet<0>(), lds);
+        if constexpr (SETS == 2) load(WgSet<1>());
         __syncthreads();
-        for (int k = 0; k < steps; ++k) {
-            u32x4* const now = lds + (k & 1) * STAGE;
-            u32x4* const next = lds + ((k & 1) ^ 1) * STAGE;
-            load(k + 1);
+        auto step = [&](int odd, auto ahead, auto behind) __attribute__((always_inline)) {      // sets of the next loads and of the next stage
+            u32x4* const now = lds + odd * STAGE + kp * BLOCK;
+            load(ahead);
             __builtin_amdgcn_sched_barrier(0);
             wg_mfma<TERMS, PLANE, FM, FN>(now, now + TERMS * PLANE, 0, wm, wn, lane, acc);
             __builtin_amdgcn_sched_barrier(0);
             wg_mfma<TERMS, PLANE, FM, FN>(now, now + TERMS * PLANE, 1, wm, wn, lane, acc);
-            put(next);
+            put(behind, lds + (odd ^ 1) * STAGE);
 #pragma unroll
             for (int i = 0; i < TERMS * FM * FN; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       // a matrix instruction,
                 __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);       // eight vector instructions in its shadow
             }
             __syncthreads();
+        };
+        if constexpr (SETS == 2) {
+            for (int k = 0; k < steps; k += 2) {
+                step(0, WgSet<0>(), WgSet<1>());
+                if (k + 1 < steps) step(1, WgSet<1>(), WgSet<0>());
+            }
+        } else {
+            for (int k = 0; k < steps; ++k) step(k & 1, WgSet<0>(), WgSet<0>());
         }
     };
-    if (wave < TM / 64) {
+    if (wave < TM * KP / 64) {
         constexpr int SZ = sizeof(T);
-        const int oct = tid / (TM / 4), col = (tid % (TM / 4)) * 4;
+        const int octs = tid / (TM / 4), oct = octs & 3, block = (octs >> 2) * BLOCK, col = (tid % (TM / 4)) * 4;
         const long first = (long)w.g * Og + m0;                          // columns behind the group's or the row's end are not stored
         const char* const from = (const char*)p.dy + (k_begin * p.O + first) * SZ;
         const unsigned lead = ODD && SZ == 2 ? (unsigned)((uintptr_t)from & 3) : 0u;      // descriptors start at a whole word
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(from) - lead, 0, (int)((((k_end - k_begin) * p.O - first) * SZ + lead + 3) & ~3L), 0x00020000);
-        const unsigned row = (unsigned)p.O * SZ, base = (unsigned)oct * 8 * row + (unsigned)col * SZ + lead;
+        const unsigned row = (unsigned)p.O * SZ, base = (unsigned)octs * 8 * row + (unsigned)col * SZ + lead;
+        unsigned at = base;                                              // of the next load's first row
         if constexpr (ODD && SZ == 2) {
-            u32x3 r[8]; unsigned odd[8];
-            loop([&](int k) {
-                     const unsigned at = base + (unsigned)k * WG_BK * row;
+            u32x3 r[SETS][8]; unsigned odd[SETS][8];
+            loop([&](auto set) __attribute__((always_inline)) {
 #pragma unroll
-                     for (int i = 0; i < 8; ++i) { const unsigned o = at + (unsigned)i * row; odd[i] = o & 2; r[i] = __builtin_amdgcn_raw_buffer_load_b96(rs, o & ~3u, 0, 0); }
+                     for (int i = 0; i < 8; ++i) { const unsigned o = at + (unsigned)i * row; odd[set.value][i] = o & 2; r[set.value][i] = __builtin_amdgcn_raw_buffer_load_b96(rs, o & ~3u, 0, 0); }
+                     at += BK * row;
                  },
-                 [&](u32x4* to) {
-                     wg_put<1, false, PLANE>(to, oct, col, [&](int i, int j) {
-                         const unsigned w = __builtin_amdgcn_alignbyte(r[i][(j >> 1) + 1], r[i][j >> 1], odd[i]);
+                 [&](auto set, u32x4* to) __attribute__((always_inline)) {
+                     wg_put<1, false, PLANE>(to + block, oct, col, [&](int i, int j) {
+                         const unsigned w = __builtin_amdgcn_alignbyte(r[set.value][i][(j >> 1) + 1], r[set.value][i][j >> 1], odd[set.value][i]);
                          return j & 1 ? bf16_hi(w) : bf16_lo(w);
                      });
                  });
         } else {
-            Raw<T, 4> r[8];
-            loop([&](int k) {
-                     const unsigned at = base + (unsigned)k * WG_BK * row;
+            Raw<T, 4> r[SETS][8];
+            loop([&](auto set) __attribute__((always_inline)) {
 #pragma unroll
-                     for (int i = 0; i < 8; ++i) r[i].load(rs, at + (unsigned)i * row);
+                     for (int i = 0; i < 8; ++i) r[set.value][i].load(rs, at + (unsigned)i * row);
+                     at += BK * row;
                  },
-                 [&](u32x4* to) {
-                     wg_put<TERMS, TERMS == 1 && SZ == 4, PLANE>(to, oct, col, [&](int i, int j) { return r[i].at(j); });
+                 [&](auto set, u32x4* to) __attribute__((always_inline)) {
+                     wg_put<TERMS, TERMS == 1 && SZ == 4, PLANE>(to + block, oct, col, [&](int i, int j) { return r[set.value][i].at(j); });
                  });
         }
     } else {
-        const int t2 = tid - TM, oct = t2 / (TN / 4), col = (t2 % (TN / 4)) * 4;
+        const int t2 = tid - TM * KP, octs = t2 / (TN / 4), oct = octs & 3, block = (octs >> 2) * BLOCK, col = (t2 % (TN / 4)) * 4;
         const WgCols cols = wg_cols(p, w.g);
         const int tap = (n0 + col) / cols.Cp, ch = n0 + col - tap * cols.Cp + cols.first;
         const bool on = tap < p.kernel && ch < p.I;
@@ -258,32 +272,54 @@ __global__ void __launch_bounds__(TM + TN) wgrad8_kernel(Wgrad8Args p, int split
         const unsigned lead = ODD ? (unsigned)((uintptr_t)from & 3) : 0u;
         const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(from) - lead, 0, (int)(((b1 - b0) * p.I + lead + 3) & ~3L), 0x00020000);
         const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.q_code + b0 * nb), 0, (int)((b1 - b0) * nb), 0x00020000);
-        const int row0 = (int)(k_begin - b0) + oct * 8 + (on ? shift : 0), step = WG_BK % p.L;
+        const int row0 = (int)(k_begin - b0) + octs * 8 + (on ? shift : 0), step = BK % p.L;
         unsigned at_q = (unsigned)(row0 * p.I + ch) + lead, at_c = (unsigned)(row0 * nb + ch / CK_BLOCK);      // of the next load's first row
-        int l0 = (int)((k_begin + oct * 8) % p.L);                       // and its place in its sample
-        unsigned q[8], c[8];
-        u32x2 wide[ODD ? 8 : 1];
-        loop([&](int) {
+        int l0 = (int)((k_begin + octs * 8) % p.L);                       // and its place in its sample
+        unsigned q[SETS][8], c[SETS][8];
+        u32x2 wide[SETS][ODD ? 8 : 1];
+        loop([&](auto set) __attribute__((always_inline)) {
+                 constexpr int S = set.value;
                  int l = l0;
 #pragma unroll
                  for (int i = 0; i < 8; ++i) {
                      const unsigned out = (unsigned)(l + shift) < (unsigned)p.L ? 0u : 0x80000000u;      // behind the end of either buffer
                      const unsigned o = at_q + (unsigned)(i * p.I);
-                     if constexpr (ODD) { wide[i] = __builtin_amdgcn_raw_buffer_load_b64(rq, (o & ~3u) | out, 0, 0); q[i] = o; }
-                     else q[i] = __builtin_amdgcn_raw_buffer_load_b32(rq, o | out, 0, 0);
-                     c[i] = __builtin_amdgcn_raw_buffer_load_b8(rc, (at_c + (unsigned)(i * nb)) | out, 0, 0);
+                     if constexpr (ODD) { wide[S][i] = __builtin_amdgcn_raw_buffer_load_b64(rq, (o & ~3u) | out, 0, 0); q[S][i] = o; }
+                     else q[S][i] = __builtin_amdgcn_raw_buffer_load_b32(rq, o | out, 0, 0);
+                     c[S][i] = __builtin_amdgcn_raw_buffer_load_b8(rc, (at_c + (unsigned)(i * nb)) | out, 0, 0);
                      l = l + 1 == p.L ? 0 : l + 1;
                  }
-                 at_q += (unsigned)(WG_BK * p.I); at_c += (unsigned)(WG_BK * nb);
+                 at_q += (unsigned)(BK * p.I); at_c += (unsigned)(BK * nb);
                  l0 += step;
                  if (l0 >= p.L) l0 -= p.L;
              },
-             [&](u32x4* to) {
+             [&](auto set, u32x4* to) __attribute__((always_inline)) {
+                 constexpr int S = set.value;
                  if constexpr (ODD)
 #pragma unroll
-                     for (int i = 0; i < 8; ++i) q[i] = __builtin_amdgcn_alignbyte(wide[i][1], wide[i][0], q[i]);
-                 wg_put<1, false, TN * 4>(to + TERMS * PLANE, oct, col, [&](int i, int j) { return ck_value((q[i] >> (8 * j)) & 0xffu, ck_scale(c[i])); });      // exact
+                     for (int i = 0; i < 8; ++i) q[S][i] = __builtin_amdgcn_alignbyte(wide[S][i][1], wide[S][i][0], q[S][i]);
+                 wg_put<1, false, TN * 4>(to + block + TERMS * PLANE, oct, col, [&](int i, int j) { return ck_value((q[S][i] >> (8 * j)) & 0xffu, ck_scale(c[S][i])); });      // exact
              });
+    }
+    if constexpr (KP > 1) {
+        static_assert(KP == 2 && FM * FN * 16 * WAVES * 64 <= 2 * STAGE * 4, "the second half's accumulators fit the stages");
+        float* const other = reinterpret_cast<float*>(lds) + (wave % WAVES) * FM * FN * 16 * 64 + lane;      // the loop ended with a barrier
+        if (kp == 1) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) other[((i * FN + j) * 16 + e) * 64] = acc[i][j][e];
+        }
+        __syncthreads();
+        if (kp == 1) return;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] += other[((i * FN + j) * 16 + e) * 64];
     }
     wg_store<FM, FN>(p, splits, w.split, w.g, m0 + wm, n0 + wn, lane, acc);
 }
@@ -342,26 +378,28 @@ static WgPlan wg_plan(const Wgrad8Args& p) {
     // quads of x and of a bf16 dy at whole words
     k.odd = p.I % 4 != 0 || !aligned_to(p.q, 4) || (sz == 2 && (p.O % 4 != 0 || Og % 4 != 0 || !aligned_to(p.dy, 8)));
     k.pipe = true;                               // offsets in a split's rows below 2^31
-    const long span = (long)(p.kernel - 1) * p.dilation + 4 * WG_BK, wide = (long)p.O * sz > p.I ? (long)p.O * sz : p.I;
+    const long span = (long)(p.kernel - 1) * p.dilation + 8 * WG_BK, wide = (long)p.O * sz > p.I ? (long)p.O * sz : p.I;
     const long most = (((1L << 31) - 8) / wide - span) / WG_BK;          // steps whose offsets fit
     if (most < 8) k.pipe = false;
     const long Nn = (long)p.kernel * wg_quad_columns(Cg);
     auto tiles = [&](long t) { return cdiv(Og, t) * (long)cdiv(Nn, t) * p.groups; };
-    auto split = [&](long t, long room) {        // `room` workgroups fill the card; at least eight steps each
-        long want = tiles(t) > room ? 1 : room / tiles(t);
+    auto split = [&](long t) {                   // one workgroup to a CU; at least eight steps each
+        long want = tiles(t) > 256 ? 1 : 256 / tiles(t);
         if (want > steps / 8) want = steps / 8;
         return want < 1 ? 1 : want;
     };
-    // 256 x 256 tiles (one to a CU) where they fill three quarters of the CUs and waste less than 0.3 of their area, 128 x 128 (two to a
-    // CU) elsewhere.  Rows, I -> O, kernel, fp32 gradients, 256 / 128, us: 38400, 512 -> 512, 5: 294 / 326; 7680: 70 / 76;
-    // 38400, kernel 1: 71 / 75; 960 (60 workgroups): 39 / 26; 38400, 256 -> 256, 1 (150 workgroups): 44 / 38; 14400, 128 -> 320, 5
-    // (0.52 of the area used): 43 / 37; 38400, 512 -> 80, 5: 130 / 90
-    const bool big = k.pipe && tiles(256) * split(256, 256) >= 192 && 10.0 * Og * Nn >= 7.0 * 65536 * (double)(tiles(256) / p.groups);
+    // 256 x 256 tiles where they fill three quarters of the CUs with sixteen steps or more each (a partial tile costs its way through
+    // memory) and waste less than 0.3 of their area, 128 x 128 of two half steps elsewhere.  Rows, I -> O,
+    // kernel, fp32 (bf16) gradients, us of 256 / 128: 38400, 512 -> 512, 5: 260 / 313 (134 / 175); 7680: 71 / 73 (46 / 47); 38400,
+    // kernel 1: 72 / 72; 38400, 127 -> 255, 3 (nine steps each): 64 / 46 (54 / 37); 1920, 512 -> 512, 5 (140 workgroups): 40 / 32;
+    // 38400, 256 -> 256, 1 (150): 45 / 32; 14400, 128 -> 320, 5 (0.52 of the area): 44 / 35; 38400, 512 -> 80, 5 (0.31): 131 / 87
+    const bool big = k.pipe && tiles(256) * split(256) >= 192 && steps >= 16 * split(256) && 10.0 * Og * Nn >= 7.0 * 65536 * (double)(tiles(256) / p.groups);
     k.tile = big ? 256 : 128;
     k.tiles_m = cdiv(Og, k.tile); k.tiles_n = cdiv(Nn, k.tile);
-    long want = big ? split(256, 256) : split(128, 512);
+    long want = split(k.tile);
     if (k.pipe && cdiv(steps, want) > most) want = cdiv(steps, most);
     k.steps_per = cdiv(steps, want);
+    if (!big && k.steps_per < steps) k.steps_per += k.steps_per & 1;      // whole double steps
     k.splits = cdiv(steps, k.steps_per);
     return k;
 }
@@ -384,20 +422,20 @@ MTTS_API long mtts_conv_weight_grad8_workspace_floats(const Wgrad8Args* args) {
     return k.splits > 1 ? (long)k.splits * args->O * args->kernel * (args->I / args->groups) : 0;
 }
 
-template <typename T, int TERMS, int TM, int TN, int WM, int WN, bool ODD> static int wg_launch(const Wgrad8Args& p, const WgPlan& k, hipStream_t s) {
-    const size_t lds = 2 * (TERMS * TM * 4 + TN * 4) * sizeof(u32x4);
-    const void* fn = (const void*)wgrad8_kernel<T, TERMS, TM, TN, WM, WN, ODD>;
+template <typename T, int TERMS, int TM, int TN, int WM, int WN, int KP, bool ODD> static int wg_launch(const Wgrad8Args& p, const WgPlan& k, hipStream_t s) {
+    const size_t lds = 2 * KP * (TERMS * TM * 4 + TN * 4) * sizeof(u32x4);
+    const void* fn = (const void*)wgrad8_kernel<T, TERMS, TM, TN, WM, WN, KP, ODD>;
     if (lds > 64 * 1024) MTTS_CHECK_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL((wgrad8_kernel<T, TERMS, TM, TN, WM, WN, ODD>), dim3(k.tiles_m * k.tiles_n * p.groups * k.splits), dim3(TM + TN), lds, s, p, k.splits, k.tiles_m, k.tiles_n, k.steps_per);
+    hipLaunchKernelGGL((wgrad8_kernel<T, TERMS, TM, TN, WM, WN, KP, ODD>), dim3(k.tiles_m * k.tiles_n * p.groups * k.splits), dim3((TM + TN) * KP), lds, s, p, k.splits, k.tiles_m, k.tiles_n, k.steps_per);
     return 0;
 }
-template <typename T, int TERMS, int TM, int TN, int WM, int WN> static int wg_pipe(const Wgrad8Args& p, const WgPlan& k, hipStream_t s) {
-    return k.odd ? wg_launch<T, TERMS, TM, TN, WM, WN, true>(p, k, s) : wg_launch<T, TERMS, TM, TN, WM, WN, false>(p, k, s);
+template <typename T, int TERMS, int TM, int TN, int WM, int WN, int KP> static int wg_pipe(const Wgrad8Args& p, const WgPlan& k, hipStream_t s) {
+    return k.odd ? wg_launch<T, TERMS, TM, TN, WM, WN, KP, true>(p, k, s) : wg_launch<T, TERMS, TM, TN, WM, WN, KP, false>(p, k, s);
 }
 template <typename T, int TERMS> static int wg_go(const Wgrad8Args& p, hipStream_t s) {
     const WgPlan k = wg_plan(p);
-    if (k.pipe && k.tile == 256) MTTS_TRY((wg_pipe<T, TERMS, 256, 256, 64, 128>(p, k, s)));
-    else if (k.pipe) MTTS_TRY((wg_pipe<T, TERMS, 128, 128, 64, 64>(p, k, s)));
+    if (k.pipe && k.tile == 256) MTTS_TRY((wg_pipe<T, TERMS, 256, 256, 64, 128, 1>(p, k, s)));
+    else if (k.pipe) MTTS_TRY((wg_pipe<T, TERMS, 128, 128, 64, 64, 2>(p, k, s)));
     else hipLaunchKernelGGL((wgrad8_edge_kernel<T, TERMS>), dim3(k.tiles_m * k.tiles_n * p.groups * k.splits), dim3(256), 0, s, p, k.splits, k.tiles_m, k.tiles_n, k.steps_per);
     if (k.splits > 1) MTTS_TRY(wg_sum(p, k.splits, s));
     MTTS_CHECK_LAUNCH("conv_weight_grad8");
