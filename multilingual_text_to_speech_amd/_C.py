@@ -162,11 +162,16 @@ def stream_ptr():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_raw_stream = None
+
+
 def stream_of(device):
     """The current stream of a tensor's device as a plain number.  (torch.cuda.current_stream() builds a Stream object: 3 us a call.)"""
-    import torch
-    raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)
-    return raw(device.index) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    return _raw_stream(device.index)
 
 
 def require_gpu(*tensors):

@@ -602,7 +602,7 @@ def _gn_fwd(x, gamma, beta, groups, lengths, mask, act, eps, mask_scale, checkpo
     N, L, C = x.shape
     dev = x.device
     y = torch.empty_like(x)
-    stats = _f32(2, N, groups, device=dev)
+    stats = torch.empty((2, N, groups), dtype=torch.float32, device=dev)
     q = code = None
     if checkpoint:
         q = torch.empty(x.shape, dtype=torch.int8, device=dev)
@@ -611,18 +611,19 @@ def _gn_fwd(x, gamma, beta, groups, lengths, mask, act, eps, mask_scale, checkpo
         at = stats.data_ptr()
         a = _C.GroupNormArgs(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _at(lengths), _at(mask), y.data_ptr(), at, at + 4 * N * groups,
                              _at(q), _at(code), None, N, L, C, groups, _DTYPE[x.dtype], act, eps, mask_scale)
-        _gn_launch('mtts_group_norm_act_fwd', a, 0, dev)
+        _gn_launch(lib().mtts_group_norm_act_fwd, 'group_norm_act_fwd', a, 0, dev)
     return y, stats, q, code
 
 
-def _gn_launch(entry, a, backward, device):
+def _gn_launch(entry, what, a, backward, device):
     at = ctypes.addressof(a)
     n = lib().mtts_group_norm_workspace_floats(at, backward)
     if n < 0:
-        _refuse(entry, lib().mtts_last_error().decode())
-    ws = _f32(n, device=device) if n else None
-    a.ws = _at(ws)
-    check(getattr(lib(), entry)(at, stream_of(device)), entry)
+        _refuse(what, lib().mtts_last_error().decode())
+    if n:
+        ws = _f32(n, device=device)
+        a.ws = ws.data_ptr()
+    check(entry(at, stream_of(device)), what)
 
 
 def _gn_bwd(x, q, code, gamma, beta, stats, lengths, mask, dy, groups, act, eps, mask_scale):
@@ -635,7 +636,7 @@ def _gn_bwd(x, q, code, gamma, beta, stats, lengths, mask, dy, groups, act, eps,
     at = stats.data_ptr()
     a = _C.GroupNormArgs(_at(x), gamma.data_ptr(), beta.data_ptr(), _at(lengths), _at(mask), None, at, at + 4 * N * groups, _at(q), _at(code), None,
                          N, L, C, groups, _DTYPE[dy.dtype], act, eps, mask_scale, dy.data_ptr(), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr())
-    _gn_launch('mtts_group_norm_act_bwd', a, 1, dy.device)
+    _gn_launch(lib().mtts_group_norm_act_bwd, 'group_norm_act_bwd', a, 1, dy.device)
     return dx, dgamma, dbeta
 
 
@@ -645,8 +646,7 @@ class GroupNormActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, lengths, mask, cfg):
         groups, act, eps, mask_scale, checkpoint = cfg
-        with _On(x.device):
-            y, stats, q, code = _gn_fwd(x, gamma, beta, groups, lengths, mask, act, eps, mask_scale, checkpoint)
+        y, stats, q, code = _gn_fwd(x, gamma, beta, groups, lengths, mask, act, eps, mask_scale, checkpoint)
         ctx.save_for_backward(None if checkpoint else x, q, code, gamma, beta, stats, lengths, mask)
         ctx.cfg = cfg
         return y
@@ -668,13 +668,16 @@ def _gn_check(what, shape, device, gamma, beta, groups, lengths, mask, act):
         _refuse(what, f'{C} channels are not a multiple of {groups} groups')
     if act not in GN_ACT:
         _refuse(what, f'unknown activation {act!r}: one of {", ".join(GN_ACT)} is expected')
-    for name, t in (('gamma', gamma), ('beta', beta)):
-        if t.dtype != torch.float32 or tuple(t.shape) != (C,):
-            _refuse(what, f'{name} is {t.dtype} {tuple(t.shape)}: float32 of shape ({C},) is expected')
+    if gamma.dtype != torch.float32 or gamma.shape != (C,):
+        _refuse(what, f'gamma is {gamma.dtype} {tuple(gamma.shape)}: float32 of shape ({C},) is expected')
+    if beta.dtype != torch.float32 or beta.shape != (C,):
+        _refuse(what, f'beta is {beta.dtype} {tuple(beta.shape)}: float32 of shape ({C},) is expected')
     if mask is not None:
-        if mask.dtype not in (torch.uint8, torch.bool) or tuple(mask.shape) != (N, L, C):
+        if mask.dtype not in (torch.uint8, torch.bool) or mask.shape != (N, L, C):
             _refuse(what, f'mask is {mask.dtype} {tuple(mask.shape)}: uint8 keep flags of shape {(N, L, C)} are expected')
-        mask = mask.contiguous().view(torch.uint8)
+        mask = mask.contiguous()
+        if mask.dtype == torch.bool:
+            mask = mask.view(torch.uint8)
     _same_device(what, device, gamma, beta, mask)
     return gamma.contiguous(), beta.contiguous(), _check_lengths(what, lengths, N, L, device), mask
 
