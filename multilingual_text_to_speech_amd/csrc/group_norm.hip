@@ -219,9 +219,9 @@ __global__ void __launch_bounds__(R > 12 ? 512 : 1024) gn_fwd_kernel(GroupNormAr
     gn_block_sums(2 * k.NG, E, [&](int g, int e) { return red[g * E + e]; }, [&](int g, float a) { stat[k.NG + g] = a * inv; });
     __syncthreads();
     if (threadIdx.x < k.NG && t.g0 + threadIdx.x < p.G) {
-        const float d = stat[k.NG + threadIdx.x], v = fmaxf(stat[2 * k.NG + threadIdx.x] - d * d, 0.f);
+        const float d = stat[k.NG + threadIdx.x], v = stat[2 * k.NG + threadIdx.x] - d * d;
         const long g = (long)t.n * p.G + t.g0 + threadIdx.x;
-        p.mean[g] = stat[threadIdx.x] + d; p.rstd[g] = 1.f / sqrtf(v + p.eps);
+        p.mean[g] = stat[threadIdx.x] + d; p.rstd[g] = 1.f / sqrtf((v < 0.f ? 0.f : v) + p.eps);      // NaN stays NaN
     }
 #pragma unroll
     for (int j = 0; j < K; ++j) {
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(GN_T) gn_moments_kernel(GroupNormArgs p, GnGeo
                 const unsigned code = ck_code(block_max<CK_BLOCK / VEC>(top));
                 const int rr = r + u * t.TY;
                 if (t.on && rr < r1) {
-                    ck_store(p.q + (first + rr) * p.C + t.c, v[u], code);
+                    ck_store(p.q + (first + rr) * p.C + t.c, v[u], code, VEC);
                     if ((t.c & (CK_BLOCK - 1)) == 0) p.q_code[(first + rr) * nb + t.c / CK_BLOCK] = (uint8_t)code;
                 }
             }

@@ -12,6 +12,9 @@ typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 
+typedef f32x4 __attribute__((aligned(4))) f32x4_at4;      // at any element
+typedef u32x4 __attribute__((aligned(2))) u32x4_at2;
+
 struct bf16_t { uint16_t v; };                 // storage type of MTTS_BF16 tensors
 
 __device__ __forceinline__ float bf16_lo(unsigned w) { return __uint_as_float(w << 16); }
@@ -22,8 +25,7 @@ __device__ __forceinline__ unsigned bf16_pack(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f, bf16x2_t));
 }
 
-// VEC values as they lie in memory: one 16-byte access (4 fp32 / 8 bf16), or one element (VEC = 1) where the width or an address does
-// not allow it.
+// VEC values as they lie in memory: one 16-byte access (4 fp32 / 8 bf16), or one element (VEC = 1).
 template <typename T, int VEC> struct Raw;
 template <> struct Raw<float, 4> {
     u32x4 w;
@@ -57,6 +59,21 @@ template <> struct Raw<bf16_t, 1> {
     __device__ __forceinline__ void zero() { w = 0; }
 };
 
+// The same from any address, and n of VEC elements (the others zero): rows of a width that is no whole number of vectors.  (The hardware
+// takes wide accesses at any byte; the compiler makes them of these copies.)
+__device__ __forceinline__ void load_any(Raw<float, 4>& r, const float* p, int n) {
+    if (n >= 4) { __builtin_memcpy(&r.w, p, 16); return; }
+    r.zero();
+#pragma unroll
+    for (int j = 0; j < 3; ++j) if (j < n) r.w[j] = __float_as_uint(p[j]);
+}
+__device__ __forceinline__ void load_any(Raw<bf16_t, 8>& r, const bf16_t* p, int n) {
+    if (n >= 8) { __builtin_memcpy(&r.w, p, 16); return; }
+    r.zero();
+#pragma unroll
+    for (int j = 0; j < 7; ++j) if (j < n) r.w[j >> 1] |= (unsigned)p[j].v << (16 * (j & 1));
+}
+
 template <typename T, int VEC> __device__ __forceinline__ void get_vec(const Raw<T, VEC>& r, float (&f)[VEC]) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) f[j] = r.at(j);
@@ -65,10 +82,21 @@ template <typename T, int VEC> __device__ __forceinline__ void get_vec(const Raw
 __device__ __forceinline__ void store_vec(float* p, const float (&f)[4]) { *reinterpret_cast<f32x4*>(p) = f32x4{f[0], f[1], f[2], f[3]}; }
 __device__ __forceinline__ void stream_vec(float* p, const float (&f)[4]) { const f32x4 v = {f[0], f[1], f[2], f[3]}; __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(p)); }
 __device__ __forceinline__ void stream_vec(float* p, const float (&f)[1]) { *p = f[0]; }
+__device__ __forceinline__ void stream_vec(bf16_t* p, const float (&f)[1]) { p->v = (uint16_t)bf16_pack(f[0], 0.f); }
+__device__ __forceinline__ void stream_any(float* p, const float (&f)[4], int n) {
+    if (n >= 4) { const f32x4 v = {f[0], f[1], f[2], f[3]}; __builtin_nontemporal_store(v, reinterpret_cast<f32x4_at4*>(p)); return; }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) if (j < n) p[j] = f[j];
+}
 __device__ __forceinline__ void store_vec(float* p, const float (&f)[1]) { *p = f[0]; }
 __device__ __forceinline__ u32x4 pack_vec(const float (&f)[8]) { return u32x4{bf16_pack(f[0], f[1]), bf16_pack(f[2], f[3]), bf16_pack(f[4], f[5]), bf16_pack(f[6], f[7])}; }
 __device__ __forceinline__ void stream_vec(bf16_t* p, const float (&f)[8]) { __builtin_nontemporal_store(pack_vec(f), reinterpret_cast<u32x4*>(p)); }
-__device__ __forceinline__ void stream_vec(bf16_t* p, const float (&f)[1]) { p->v = (uint16_t)bf16_pack(f[0], 0.f); }
+__device__ __forceinline__ void stream_any(bf16_t* p, const float (&f)[8], int n) {
+    const u32x4 v = pack_vec(f);
+    if (n >= 8) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4_at2*>(p)); return; }
+#pragma unroll
+    for (int j = 0; j < 7; ++j) if (j < n) p[j].v = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
+}
 __device__ __forceinline__ void stream_vec(__amdgpu_buffer_rsrc_t r, unsigned at, const float (&f)[4]) {
     __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])}, r, at, 0, BUF_NT);
 }
@@ -97,6 +125,19 @@ template <> struct Bytes<8> {
     __device__ __forceinline__ void fill(unsigned v) { w = u32x2{v * 0x01010101u, v * 0x01010101u}; }
 };
 
+__device__ __forceinline__ void load_any(Bytes<4>& r, const void* p, int n) {
+    if (n >= 4) { __builtin_memcpy(&r.w, p, 4); return; }
+    r.w = 0;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) if (j < n) r.w |= (unsigned)((const uint8_t*)p)[j] << (8 * j);
+}
+__device__ __forceinline__ void load_any(Bytes<8>& r, const void* p, int n) {
+    if (n >= 8) { __builtin_memcpy(&r.w, p, 8); return; }
+    r.w = u32x2{0, 0};
+#pragma unroll
+    for (int j = 0; j < 7; ++j) if (j < n) r.w[j >> 2] |= (unsigned)((const uint8_t*)p)[j] << (8 * (j & 3));
+}
+
 // ---- 8-bit checkpoint: blocks of 32 channels of a row, value = q * 2^(code - 127) -----------------------------------------------------
 // code is the smallest exponent that keeps |round(x / s)| <= 127: with amax = m 2^k, m in [1, 2), amax / 2^(k-6) = 64 m rounds to 128
 // exactly when m >= 255/128, i.e. when adding 0x10000 to amax's bits carries into the exponent.  code >= 1 (s >= 2^-126, a normal
@@ -122,8 +163,19 @@ template <typename R> __device__ __forceinline__ unsigned ck_word(const R& x, in
     for (int j = 0; j < 4; ++j) w |= ((unsigned)ck_quantise(x.at(4 * h + j), code) & 0xffu) << (8 * j);
     return w;
 }
-__device__ __forceinline__ void ck_store(int8_t* q, const Raw<float, 4>& x, unsigned code) { *reinterpret_cast<unsigned*>(q) = ck_word(x, 0, code); }
-__device__ __forceinline__ void ck_store(int8_t* q, const Raw<bf16_t, 8>& x, unsigned code) { *reinterpret_cast<u32x2*>(q) = u32x2{ck_word(x, 0, code), ck_word(x, 1, code)}; }
+// n of the vector's values, to any address
+__device__ __forceinline__ void ck_store(int8_t* q, const Raw<float, 4>& x, unsigned code, int n) {
+    const unsigned w = ck_word(x, 0, code);
+    if (n >= 4) { __builtin_memcpy(q, &w, 4); return; }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) if (j < n) q[j] = (int8_t)(w >> (8 * j));
+}
+__device__ __forceinline__ void ck_store(int8_t* q, const Raw<bf16_t, 8>& x, unsigned code, int n) {
+    const u32x2 w = {ck_word(x, 0, code), ck_word(x, 1, code)};
+    if (n >= 8) { __builtin_memcpy(q, &w, 8); return; }
+#pragma unroll
+    for (int j = 0; j < 7; ++j) if (j < n) q[j] = (int8_t)(w[j >> 2] >> (8 * (j & 3)));
+}
 __device__ __forceinline__ void ck_store(__amdgpu_buffer_rsrc_t r, unsigned at, const Raw<float, 4>& x, unsigned code) {
     __builtin_amdgcn_raw_buffer_store_b32(ck_word(x, 0, code), r, at, 0, 0);      // 32-byte pieces of a line, gathered in L2: 44 -> 36 us for the call
 }

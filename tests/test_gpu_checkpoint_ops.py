@@ -62,7 +62,8 @@ def check_norm(x, gamma, beta, keep, dy, lens, G, act, ckpt, scale=1.0, eps=1e-5
 # the widths of the encoder and the post-net, long samples, more rows than a workgroup keeps
 SHAPES = [(1, 1, 512, 32), (1, 1, 8, 1), (3, 7, 80, 8), (2, 13, 37, 1), (2, 9, 35, 5), (2, 50, 6, 6), (4, 33, 12, 2), (5, 120, 512, 32),
           (2, 600, 512, 16), (2, 257, 96, 3), (1, 1500, 64, 4), (1, 5000, 40, 2), (3, 431, 80, 8), (2, 65, 2560, 10), (1, 70, 4100, 2),
-          (2, 1025, 128, 4), (1, 2049, 256, 2), (70, 3, 64, 2), (2, 31, 1024, 1)]
+          (2, 1025, 128, 4), (1, 2049, 256, 2), (70, 3, 64, 2), (2, 31, 1024, 1),
+          (2, 600, 511, 7), (3, 90, 515, 1), (2, 40, 2058, 2), (2, 33, 9000, 8), (1, 20, 4101, 1), (3, 64, 1, 1), (2, 100, 84, 4), (5, 17, 1030, 2)]
 
 
 @pytest.mark.parametrize('ckpt', [False, True])
@@ -115,6 +116,12 @@ def test_a_non_finite_value_stays_in_its_group():
     hit = torch.zeros_like(x, dtype=torch.bool)
     hit[1, :, 16:32] = True
     assert y[hit].isnan().all() and torch.equal(y[~hit], clean[~hit])
+    for L in (50, 3000):                         # one workgroup to a strip, two passes
+        xs = x.repeat(1, L // 50, 1).requires_grad_()
+        for act in ('identity', 'relu', 'silu'):
+            dx, = torch.autograd.grad(K.group_norm_act(xs, gamma, beta, 4, act=act), xs, dy.repeat(1, L // 50, 1))
+            at = hit.repeat(1, L // 50, 1)
+            assert dx[at].isnan().all() and torch.isfinite(dx[~at]).all()
 
 
 @pytest.mark.parametrize('offset', [100.0, 3000.0])
