@@ -85,7 +85,7 @@ def _linear_bwd8(held, weight, dy, need_dx):
     """linear_bwd with the input held as a Checkpoint8."""
     N, K = weight.shape
     dy2 = dy.reshape(-1, N)
-    dW = conv1d_weight_grad8(Checkpoint8(held.values.view(-1, K), held.scales.view(dy2.shape[0], -1)), dy2, 1).view(N, K)
+    dW = conv1d_weight_grad8(Checkpoint8._of(held.values.view(-1, K), held.scales.view(dy2.shape[0], -1)), dy2, 1).view(N, K)
     db = colsum(dy2)
     dx = None
     if need_dx:
@@ -122,7 +122,7 @@ class LinearFn(torch.autograd.Function):
         elif ctx.act != 0:
             raise NotImplementedError('LinearFn backward supports identity/relu')
         if ctx.checkpoint:
-            dx, dW, db = _linear_bwd8(Checkpoint8(x, scales), weight, dz, ctx.needs_input_grad[0])
+            dx, dW, db = _linear_bwd8(Checkpoint8._of(x, scales), weight, dz, ctx.needs_input_grad[0])
         else:
             dx, dW, db = linear_bwd(x, weight, dz, ctx.needs_input_grad[0])
         return dx, dW, (db if ctx.has_bias else None), None, None, None, None
@@ -383,8 +383,8 @@ class ConvBnActFn(torch.autograd.Function):
         packed = len(ctx.cfg) > 9 and ctx.cfg[9]
         held_x = None
         if ctx.checkpoint:
-            held_x = Checkpoint8(x, x_scales)
-            conv = Checkpoint8(conv, conv_scales).unpack()
+            held_x = Checkpoint8._of(x, x_scales)
+            conv = Checkpoint8._of(conv, conv_scales).unpack()
             x = held_x.unpack() if highway else x
         N_, L, Cin = x.shape
         O = conv.shape[2]
@@ -503,12 +503,19 @@ class Checkpoint8:
         if values.dtype != torch.int8 or scales.dtype != torch.uint8 or values.dim() < 1:
             _refuse('Checkpoint8', f'values {values.dtype}, scales {scales.dtype}: int8 and uint8 are expected')
         want = (*values.shape[:-1], -(-values.shape[-1] // CHECKPOINT_BLOCK))
-        if tuple(scales.shape) != want:
+        if scales.shape != want:
             _refuse('Checkpoint8', f'scales have shape {tuple(scales.shape)}: {want} is expected for values of shape {tuple(values.shape)}')
         if dtype not in _DTYPE:
             _refuse('Checkpoint8', f'dtype is {dtype}: float32 or bfloat16 is expected')
         _same_device('Checkpoint8', values.device, scales)
         self.values, self.scales, self.dtype = values.contiguous(), scales.contiguous(), dtype
+
+    @classmethod
+    def _of(cls, values, scales, dtype=torch.float32):
+        """Around tensors that this module made: nothing to check."""
+        held = cls.__new__(cls)
+        held.values, held.scales, held.dtype = values, scales, dtype
+        return held
 
     @property
     def shape(self):
@@ -548,7 +555,8 @@ def checkpoint8(x, lengths=None):
     if x.numel() // x.shape[-1] > _MOST_ROWS:
         _refuse(what, f'{x.numel() // x.shape[-1]} rows are too many for one call')
     require_gpu(x)
-    x = x.detach().contiguous()
+    if not x.is_contiguous():
+        x = x.detach().contiguous()
     C = x.shape[-1]
     values = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scales = torch.empty((*x.shape[:-1], -(-C // CHECKPOINT_BLOCK)), dtype=torch.uint8, device=x.device)
@@ -557,7 +565,7 @@ def checkpoint8(x, lengths=None):
         with _On(x.device):
             lens = _device_lengths(what, lengths, x.device)
             check(lib().mtts_checkpoint8_pack(x.data_ptr(), _at(lens), values.data_ptr(), scales.data_ptr(), N, L, C, _DTYPE[x.dtype], stream_of(x.device)), what)
-    return Checkpoint8(values, scales, x.dtype)
+    return Checkpoint8._of(values, scales, x.dtype)
 
 
 def conv1d_weight_grad8(held, dy, kernel, dilation=1, groups=1, packed=False):
@@ -582,7 +590,8 @@ def conv1d_weight_grad8(held, dy, kernel, dilation=1, groups=1, packed=False):
     rows = dy.numel() // O
     if not rows:
         return torch.zeros(shape, dtype=torch.float32, device=dy.device)
-    dy = dy.detach().contiguous()
+    if not dy.is_contiguous():
+        dy = dy.detach().contiguous()
     dw = _f32(shape, device=dy.device)
     N, L = (dy.shape[0], dy.shape[1]) if kernel > 1 else (1, rows)
     a = _C.Wgrad8Args(held.values.data_ptr(), held.scales.data_ptr(), dy.data_ptr(), dw.data_ptr(), None, N, L, I, O, kernel, dilation, groups,
@@ -731,7 +740,7 @@ class ConvGnActFn(torch.autograd.Function):
             need_dx = ctx.needs_input_grad[0]
             if checkpoint:
                 dx = conv1d_input_grad(wp, dconv, x.shape[2], k, dilation, groups) if need_dx else None
-                dw = conv1d_weight_grad8(Checkpoint8(x, x_scales), dconv, k, dilation, groups)
+                dw = conv1d_weight_grad8(Checkpoint8._of(x, x_scales), dconv, k, dilation, groups)
             else:
                 dx, dwp = conv1d_bwd(x, wp, dconv, k, dilation, groups, need_dx)
                 dw = unpack_conv_weight(dwp, *ctx.wshape)
