@@ -8,10 +8,11 @@
 // the leading eight bits of what is left (an exact split, 24 bits), against six where both operands are fp32.  fp32 accumulation.
 // A bf16 gradient, and an fp32 one in bf16 mode (rounded to nearest even), takes one term.
 //
-// What bounds it: the matrix pipes.  At 38400 rows, 512 -> 512 channels, kernel 5 (100.7 GFLOP, three terms) the whole call takes 243 us,
+// What bounds it: the matrix pipes.  At 38400 rows, 512 -> 512 channels, kernel 5 (100.7 GFLOP, three terms) the whole call takes 244 us,
 // 1240 TFLOP/s of bf16 products where a plain bf16 library product of 8192^3 reaches 1330 on the same card.  One term (bf16 gradients):
-// 134 us, LDS traffic beside the matrix pipes.  At 7680 rows, bf16 (20 GFLOP) 46 us: half of that is the partial tiles' way through
-// memory (63 MB out and in at twelve splits).
+// 120 us, 840 TFLOP/s: a step's 1024 cycles of matrix instructions stand beside 1024 cycles of LDS reads and writes (at 128 bytes a
+// cycle) and 900 of vector instructions, two thirds of them for the checkpoint.  At 7680 rows, bf16 (20 GFLOP) 48 us: half of that is
+// the partial tiles' way through memory (63 MB out and in at twelve splits).
 //
 // Tile TM x TN x 32 rows per workgroup, v_mfma_f32_32x32x16_bf16.  A thread takes 8 rows x 4 columns: the transposition happens in
 // registers, and 8 rows of one column are the 16 bytes that a lane feeds to the matrix instruction.  LDS holds these 16-byte units in
@@ -209,13 +210,12 @@ __global__ void __launch_bounds__((TM + TN) * KP) wgrad8_kernel(Wgrad8Args p, in
             load(ahead);
             __builtin_amdgcn_sched_barrier(0);
             wg_mfma<TERMS, PLANE, FM, FN>(now, now + TERMS * PLANE, 0, wm, wn, lane, acc);
-            __builtin_amdgcn_sched_barrier(0);
             wg_mfma<TERMS, PLANE, FM, FN>(now, now + TERMS * PLANE, 1, wm, wn, lane, acc);
             put(behind, lds + (odd ^ 1) * STAGE);
 #pragma unroll
-            for (int i = 0; i < TERMS * FM * FN; ++i) {
+            for (int i = 0; i < 2 * TERMS * FM * FN; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       // a matrix instruction,
-                __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);       // eight vector instructions in its shadow
+                __builtin_amdgcn_sched_group_barrier(0x002, 12, 0);      // twelve vector instructions beside it (eight, second half only: 125 against 120 us in bf16)
             }
             __syncthreads();
         };
@@ -327,13 +327,13 @@ __global__ void __launch_bounds__((TM + TN) * KP) wgrad8_kernel(Wgrad8Args p, in
 // dw = sum over the splits, in split order; slabs [O, kernel, Cg] -> the same (packed) or [O, Cg, kernel].  A workgroup takes one output
 // channel and CC input channels with all their taps: the sums cross over in LDS, so that reads and writes are both contiguous.
 template <int VEC>
-__global__ void __launch_bounds__(256) wgrad8_sum_kernel(Wgrad8Args p, int splits, int CC, int chunks) {
+__global__ void __launch_bounds__(512) wgrad8_sum_kernel(Wgrad8Args p, int splits, int CC, int chunks) {
     extern __shared__ float tile[];          // [CC][kernel]
     const int Cg = p.I / p.groups, k = p.kernel, Nn = k * Cg;
     const int o = blockIdx.x / chunks, c0 = (blockIdx.x - o * chunks) * CC, cc = min(CC, Cg - c0), quads = (cc + VEC - 1) / VEC;
     const long slab = (long)p.O * Nn;
     const float* const ws = p.ws + (long)o * Nn + c0;
-    for (int i = threadIdx.x; i < quads * k; i += 256) {
+    for (int i = threadIdx.x; i < quads * k; i += blockDim.x) {
         const int t = i / quads, c = (i - t * quads) * VEC;
         float s[VEC];
 #pragma unroll
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(256) wgrad8_sum_kernel(Wgrad8Args p, int split
     }
     if (p.packed) return;
     __syncthreads();
-    for (int i = threadIdx.x; i < cc * k; i += 256) p.dw[(long)o * Nn + (long)c0 * k + i] = tile[i];
+    for (int i = threadIdx.x; i < cc * k; i += blockDim.x) p.dw[(long)o * Nn + (long)c0 * k + i] = tile[i];
 }
 static int wg_sum(const Wgrad8Args& p, int splits, hipStream_t s) {
     const int Cg = p.I / p.groups;
@@ -365,8 +365,10 @@ static int wg_sum(const Wgrad8Args& p, int splits, hipStream_t s) {
     const bool v = Cg % 4 == 0 && CC % 4 == 0 && aligned_to(p.ws, 16) && (!p.packed || aligned_to(p.dw, 16));
     const size_t lds = p.packed ? 0 : (size_t)CC * p.kernel * 4;
     const dim3 grid((unsigned)((long)p.O * chunks));
-    if (v) hipLaunchKernelGGL(wgrad8_sum_kernel<4>, grid, dim3(256), lds, s, p, splits, CC, chunks);
-    else hipLaunchKernelGGL(wgrad8_sum_kernel<1>, grid, dim3(256), lds, s, p, splits, CC, chunks);
+    // a vector per thread where 512 hold them: 127 -> 255 channels, kernel 3, 28 splits: 36.2 -> 33.2 us for the whole call
+    const int vectors = (Cg < CC ? Cg : CC) * p.kernel / (v ? 4 : 1), threads = vectors >= 512 ? 512 : (vectors + 63) & ~63;
+    if (v) hipLaunchKernelGGL(wgrad8_sum_kernel<4>, grid, dim3(threads), lds, s, p, splits, CC, chunks);
+    else hipLaunchKernelGGL(wgrad8_sum_kernel<1>, grid, dim3(threads), lds, s, p, splits, CC, chunks);
     return 0;
 }
 
@@ -390,7 +392,7 @@ static WgPlan wg_plan(const Wgrad8Args& p) {
     };
     // 256 x 256 tiles where they fill three quarters of the CUs with sixteen steps or more each (a partial tile costs its way through
     // memory) and waste less than 0.3 of their area, 128 x 128 of two half steps elsewhere.  Rows, I -> O,
-    // kernel, fp32 (bf16) gradients, us of 256 / 128: 38400, 512 -> 512, 5: 260 / 313 (134 / 175); 7680: 71 / 73 (46 / 47); 38400,
+    // kernel, fp32 (bf16) gradients, us of 256 / 128: 38400, 512 -> 512, 5: 245 / 302 (120 / 178); 7680: 69 / 72 (47 / 49); 38400,
     // kernel 1: 72 / 72; 38400, 127 -> 255, 3 (nine steps each): 64 / 46 (54 / 37); 1920, 512 -> 512, 5 (140 workgroups): 40 / 32;
     // 38400, 256 -> 256, 1 (150): 45 / 32; 14400, 128 -> 320, 5 (0.52 of the area): 44 / 35; 38400, 512 -> 80, 5 (0.31): 131 / 87
     const bool big = k.pipe && tiles(256) * split(256) >= 192 && steps >= 16 * split(256) && 10.0 * Og * Nn >= 7.0 * 65536 * (double)(tiles(256) / p.groups);
