@@ -660,31 +660,54 @@ __global__ void __launch_bounds__(GN_T) gn_bwd_apply_kernel(GroupNormArgs p, GnG
     }
 }
 
-// dgamma, dbeta: sums over the rows of ws[2][rows][C] in row order.  grid ceil(C / 64), block 64 x 16
-__global__ void __launch_bounds__(1024) gn_param_grad_kernel(const float* __restrict__ ws, float* __restrict__ dgamma, float* __restrict__ dbeta, long rows, int C) {
+// Sums over the rows of ws[2][rows][C] in row order, every `stride`-th row of a piece: into the piece's first row, or (TO_GRAD, one piece)
+// into dgamma and dbeta.  grid (ceil(C / 64), pieces), block 64 x 16
+constexpr int GN_PIECE = 256;
+template <bool TO_GRAD>
+__global__ void __launch_bounds__(1024) gn_param_grad_kernel(float* ws, float* __restrict__ dgamma, float* __restrict__ dbeta, long rows, int C, long piece, int stride) {
     __shared__ float s1[16][64], s2[16][64];
     const int c = blockIdx.x * 64 + threadIdx.x;
+    const long first = blockIdx.y * piece * stride, n = min(piece, (rows - first + stride - 1) / stride);
+    float* const w1 = ws + first * C + c;
+    float* const w2 = w1 + rows * C;
     float a = 0.f, b = 0.f;
     if (c < C)
-        for (long r = threadIdx.y; r < rows; r += 16 * 8) {
+        for (long r = threadIdx.y; r < n; r += 16 * 8) {
             float u[8], v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const long rr = r + 16 * i < rows ? r + 16 * i : rows - 1;
-                u[i] = ws[rr * C + c]; v[i] = ws[(rows + rr) * C + c];
+                const long rr = (r + 16 * i < n ? r + 16 * i : n - 1) * stride;
+                u[i] = w1[rr * C]; v[i] = w2[rr * C];
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (r + 16 * i < rows) { a += u[i]; b += v[i]; }
+                if (r + 16 * i < n) { a += u[i]; b += v[i]; }
         }
     s1[threadIdx.y][threadIdx.x] = a; s2[threadIdx.y][threadIdx.x] = b;
-    __syncthreads();
+    __syncthreads();                             // every row of the piece has been read
     if (threadIdx.y == 0 && c < C) {
 #pragma unroll
         for (int i = 1; i < 16; ++i) { a += s1[i][threadIdx.x]; b += s2[i][threadIdx.x]; }
-        if (dbeta) dbeta[c] = a;
-        if (dgamma) dgamma[c] = b;
+        if constexpr (TO_GRAD) {
+            if (dbeta) dbeta[c] = a;
+            if (dgamma) dgamma[c] = b;
+        } else {
+            *w1 = a; *w2 = b;
+        }
     }
+}
+// One launch for up to 1024 rows, else pieces first: whole backward at 4096 samples of 16 rows, 512 channels 138 -> 106 us, at 4096 x 16 x 64
+// 56 -> 22 us, at 1200 x 1 x 512 33 -> 25 us.
+static int gn_param_grad(const GroupNormArgs& p, long rows, hipStream_t s) {
+    const int tiles = cdiv(p.C, 64);
+    int stride = 1;
+    if (rows > 4 * GN_PIECE) {
+        const long pieces = (rows + GN_PIECE - 1) / GN_PIECE;
+        hipLaunchKernelGGL(gn_param_grad_kernel<false>, dim3(tiles, (unsigned)pieces), dim3(64, 16), 0, s, p.ws, nullptr, nullptr, rows, p.C, (long)GN_PIECE, 1);
+        stride = GN_PIECE;
+    }
+    hipLaunchKernelGGL(gn_param_grad_kernel<true>, dim3(tiles), dim3(64, 16), 0, s, p.ws, p.dgamma, p.dbeta, rows, p.C, rows, stride);
+    return 0;
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
@@ -865,8 +888,7 @@ MTTS_API int mtts_group_norm_act_bwd(const GroupNormArgs* args, void* stream) {
         else if (k.str) MTTS_TRY((gn_bwd_any<bf16_t, 8, true>(p, k, s)));
         else MTTS_TRY((gn_bwd_any<bf16_t, 8, false>(p, k, s)));
     }
-    if (p.dgamma || p.dbeta)
-        hipLaunchKernelGGL(gn_param_grad_kernel, dim3(cdiv(p.C, 64)), dim3(64, 16), 0, s, p.ws, p.dgamma, p.dbeta, (long)p.N * k.geo.chunks, p.C);
+    if (p.dgamma || p.dbeta) MTTS_TRY(gn_param_grad(p, (long)p.N * k.geo.chunks, s));
     MTTS_CHECK_LAUNCH("group_norm_act_bwd");
     return 0;
 }

@@ -59,11 +59,12 @@ def check_norm(x, gamma, beta, keep, dy, lens, G, act, ckpt, scale=1.0, eps=1e-5
 
 
 # (N, L, C, G): one row, one value to a group's channel count, odd widths, vectors that straddle groups, one group, one channel per group,
-# the widths of the encoder and the post-net, long samples, more rows than a workgroup keeps
+# the widths of the encoder and the post-net, long samples, more rows than a workgroup keeps, more samples than one pass of the sums takes
 SHAPES = [(1, 1, 512, 32), (1, 1, 8, 1), (3, 7, 80, 8), (2, 13, 37, 1), (2, 9, 35, 5), (2, 50, 6, 6), (4, 33, 12, 2), (5, 120, 512, 32),
           (2, 600, 512, 16), (2, 257, 96, 3), (1, 1500, 64, 4), (1, 5000, 40, 2), (3, 431, 80, 8), (2, 65, 2560, 10), (1, 70, 4100, 2),
           (2, 1025, 128, 4), (1, 2049, 256, 2), (70, 3, 64, 2), (2, 31, 1024, 1),
-          (2, 600, 511, 7), (3, 90, 515, 1), (2, 40, 2058, 2), (2, 33, 9000, 8), (1, 20, 4101, 1), (3, 64, 1, 1), (2, 100, 84, 4), (5, 17, 1030, 2)]
+          (2, 600, 511, 7), (3, 90, 515, 1), (2, 40, 2058, 2), (2, 33, 9000, 8), (1, 20, 4101, 1), (3, 64, 1, 1), (2, 100, 84, 4), (5, 17, 1030, 2),
+          (1025, 2, 64, 2), (1801, 1, 70, 5)]
 
 
 @pytest.mark.parametrize('ckpt', [False, True])
