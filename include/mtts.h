@@ -809,7 +809,9 @@ float mtts_prof_empty_ms(void);
 long mtts_gemm_planes_count(void);
 
 const char* mtts_last_error(void);
-/* ABI version.  102 (round 6): DecoderGradArgs gained part_ring / part_ring_slots; new exports mtts_decoder_bwd_ring_slots,
+/* ABI version.  103: new exports mtts_group_norm_act_fwd / _bwd, mtts_group_norm_workspace_floats, mtts_checkpoint8_pack / _unpack,
+ * mtts_conv_weight_grad8, mtts_conv_weight_grad8_workspace_floats with GroupNormArgs and Wgrad8Args, MTTS_ACT_SILU; nothing else moved.
+ * 102 (round 6): DecoderGradArgs gained part_ring / part_ring_slots; new exports mtts_decoder_bwd_ring_slots,
  * mtts_set_planes_workspace, mtts_planes_trim, mtts_debug_occupy.  101 (round 5) is NOT layout-compatible with 100: AdamArgs gained `guard`, LstmPackArgs lost `plain_rows`, AttnBwdArgs
  * lost `hsum_out` / `hsum_cols`, DecoderGradArgs lost three fields, the mtts_ksplit_* exports are gone, LstmStepArgs.precision takes 2
  * (pre-split planes), DecoderArgs gained the long-input fields of the persistent decoder.  Bindings that do not generate their structs
@@ -818,7 +820,7 @@ int mtts_version(void);
 /* Bitmask of compile-time switches that make a build compute WRONG results on purpose (timing experiments).  The product sources
  * have none left (round 4); always 0 - bindings keep refusing anything else. */
 int mtts_build_flags(void);
-/* sizeof() of the structs above in declaration order (0 = GemmArgs ... 6 = BiLstmArgs, 7 = AttnBwdArgs, 8 = DecoderGradArgs, 9 = BiLstmGradArgs, 10 = TacoLossArgs, 11 = AdamArgs, 12 = LstmPackArgs, 13 = LstmStepArgs, 14 = GenParamsArgs); -1 when out of range */
+/* sizeof() of the structs above in declaration order (0 = GemmArgs ... 6 = BiLstmArgs, 7 = AttnBwdArgs, 8 = DecoderGradArgs, 9 = BiLstmGradArgs, 10 = TacoLossArgs, 11 = AdamArgs, 12 = LstmPackArgs, 13 = LstmStepArgs, 14 = GenParamsArgs, 16 = GroupNormArgs, 17 = Wgrad8Args); -1 when out of range */
 int mtts_sizeof_struct(int which);
 
 
