@@ -326,7 +326,7 @@ __global__ void __launch_bounds__((TM + TN) * KP) wgrad8_kernel(Wgrad8Args p, in
 
 // dw = sum over the splits, in split order; slabs [O, kernel, Cg] -> the same (packed) or [O, Cg, kernel].  A workgroup takes one output
 // channel and CC input channels with all their taps: the sums cross over in LDS, so that reads and writes are both contiguous.
-template <int VEC>
+template <int VEC, int U>
 __global__ void __launch_bounds__(512) wgrad8_sum_kernel(Wgrad8Args p, int splits, int CC, int chunks) {
     extern __shared__ float tile[];          // [CC][kernel]
     const int Cg = p.I / p.groups, k = p.kernel, Nn = k * Cg;
@@ -338,12 +338,12 @@ __global__ void __launch_bounds__(512) wgrad8_sum_kernel(Wgrad8Args p, int split
         float s[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s[j] = 0.f;
-        for (int k0 = 0; k0 < splits; k0 += 4) {                         // four slabs requested per round trip, added in slab order
-            Raw<float, VEC> v[4];
+        for (int k0 = 0; k0 < splits; k0 += U) {                         // U slabs requested per round trip, added in slab order
+            Raw<float, VEC> v[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u].load(ws + min(k0 + u, splits - 1) * slab + (long)t * Cg + c);
+            for (int u = 0; u < U; ++u) v[u].load(ws + min(k0 + u, splits - 1) * slab + (long)t * Cg + c);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < U; ++u)
                 if (k0 + u < splits)
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) s[j] += v[u].at(j);
@@ -365,10 +365,12 @@ static int wg_sum(const Wgrad8Args& p, int splits, hipStream_t s) {
     const bool v = Cg % 4 == 0 && CC % 4 == 0 && aligned_to(p.ws, 16) && (!p.packed || aligned_to(p.dw, 16));
     const size_t lds = p.packed ? 0 : (size_t)CC * p.kernel * 4;
     const dim3 grid((unsigned)((long)p.O * chunks));
-    // a vector per thread where 512 hold them: 127 -> 255 channels, kernel 3, 28 splits: 36.2 -> 33.2 us for the whole call
+    // Sixteen slabs a round trip where there are more: 38400 rows, 64 -> 64 channels, kernel 3 (128 slabs): 29.6 -> 24.2 us for the whole call.
+    // A vector per thread where 512 hold them: 127 -> 255 channels, kernel 3, 28 splits: 36.2 -> 33.2 us for the whole call
     const int vectors = (Cg < CC ? Cg : CC) * p.kernel / (v ? 4 : 1), threads = vectors >= 512 ? 512 : (vectors + 63) & ~63;
-    if (v) hipLaunchKernelGGL(wgrad8_sum_kernel<4>, grid, dim3(threads), lds, s, p, splits, CC, chunks);
-    else hipLaunchKernelGGL(wgrad8_sum_kernel<1>, grid, dim3(threads), lds, s, p, splits, CC, chunks);
+    if (v && splits > 16) hipLaunchKernelGGL((wgrad8_sum_kernel<4, 16>), grid, dim3(threads), lds, s, p, splits, CC, chunks);
+    else if (v) hipLaunchKernelGGL((wgrad8_sum_kernel<4, 4>), grid, dim3(threads), lds, s, p, splits, CC, chunks);
+    else hipLaunchKernelGGL((wgrad8_sum_kernel<1, 16>), grid, dim3(threads), lds, s, p, splits, CC, chunks);
     return 0;
 }
 
@@ -385,11 +387,13 @@ static WgPlan wg_plan(const Wgrad8Args& p) {
     if (most < 8) k.pipe = false;
     const long Nn = (long)p.kernel * wg_quad_columns(Cg);
     auto tiles = [&](long t) { return cdiv(Og, t) * (long)cdiv(Nn, t) * p.groups; };
-    auto split = [&](long t) {                   // one workgroup to a CU; at least eight steps each
+    auto split = [&](long t) {                   // one workgroup to a CU; at least six steps each
         long want = tiles(t) > 256 ? 1 : 256 / tiles(t);
-        if (want > steps / 8) want = steps / 8;
+        if (want > steps / 6) want = steps / 6;
         return want < 1 ? 1 : want;
     };
+    // Six steps at least: 1030 rows, 49 -> 199 channels, kernel 1: 15.7 us, with eight 17.0, four 14.7; 7777 rows, 122 -> 97, kernel 3, bf16:
+    // 16.7, 17.3, 19; 256 rows, 512 -> 512, kernel 5 (eight steps in all): 14.6, 14.6, 18.
     // 256 x 256 tiles where they fill three quarters of the CUs with sixteen steps or more each (a partial tile costs its way through
     // memory) and waste less than 0.3 of their area, 128 x 128 of two half steps elsewhere.  Rows, I -> O,
     // kernel, fp32 (bf16) gradients, us of 256 / 128: 38400, 512 -> 512, 5: 245 / 302 (120 / 178); 7680: 69 / 72 (47 / 49); 38400,
