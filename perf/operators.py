@@ -241,10 +241,10 @@ def _exact_round_trip(x):
     for c in range(0, C, BLOCK):
         b = x[:, c:c + BLOCK]
         top = b.abs().amax(1, keepdim=True)
-        e = (torch.frexp(top)[1] - 7).clamp_min(-126).long()
-        step = ((e + 1023) << 52).view(torch.float64)
-        step = torch.where(torch.round(top / step) > 127, 2 * step, step)
-        out[:, c:c + BLOCK] = torch.round(b / step) * step
+        e = torch.frexp(top)[1] - 7
+        e = e + (torch.round(torch.ldexp(top, -e)) > 127).to(e.dtype)
+        e = e.clamp_min(-126)
+        out[:, c:c + BLOCK] = torch.ldexp(torch.round(torch.ldexp(b, -e)), e)
     return out
 
 
