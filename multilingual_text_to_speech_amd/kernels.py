@@ -7,6 +7,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _C
 from ._C import check, lib, ptr, require_gpu, stream_of, stream_ptr
@@ -442,6 +443,12 @@ def _first_derivative_only(what):
         _refuse(what, 'there is no second derivative (create_graph=True)')
 
 
+def _differentiated(*tensors):
+    """Whether autograd follows the call: a graph is being recorded, or an operand carries a forward-mode tangent (such an operand need
+    not require a gradient; autograd.Function refuses it where there is no jvp)."""
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _same_device(what, device, *tensors):
     for t in tensors:
         if t is not None and t.device != device:
@@ -707,7 +714,7 @@ def group_norm_act(x, gamma, beta, groups, lengths=None, mask=None, *, act='iden
     require_gpu(x)
     with _On(x.device):
         lens, x = _device_lengths(what, lengths, x.device), x.contiguous()
-        if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
+        if _differentiated(x, gamma, beta):
             return GroupNormActFn.apply(x, gamma, beta, lens, mask, (groups, GN_ACT[act], eps, mask_scale, checkpoint))
         return _gn_fwd(x, gamma, beta, groups, lens, mask, GN_ACT[act], eps, mask_scale, False)[0]
 
