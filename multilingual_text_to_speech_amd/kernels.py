@@ -86,7 +86,7 @@ def _linear_bwd8(held, weight, dy, need_dx):
     """linear_bwd with the input held as a Checkpoint8."""
     N, K = weight.shape
     dy2 = dy.reshape(-1, N)
-    dW = conv1d_weight_grad8(Checkpoint8._of(held.values.view(-1, K), held.scales.view(dy2.shape[0], -1)), dy2, 1).view(N, K)
+    dW = conv1d_weight_grad8(Checkpoint8._of(held.values.view(-1, K), held.scales.view(-1, held.scales.shape[-1])), dy2, 1).view(N, K)
     db = colsum(dy2)
     dx = None
     if need_dx:

@@ -27,3 +27,17 @@ def test_a_forward_mode_tangent_is_refused(dual, recording):
             K.group_norm_act(t['x'], t['gamma'], t['beta'], 4, act='silu')
         with pytest.raises(RuntimeError, match='jvp'):
             K.linear(forward_ad.make_dual(w, w), w)
+
+
+# ---- empty inputs ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('shape', [(0, 80), (3, 0, 80)], ids=str)
+@pytest.mark.parametrize('act', ['identity', 'relu'])
+def test_linear_of_no_rows_from_a_checkpoint(shape, act):
+    x, w, b = (torch.randn(*s, device=DEV, requires_grad=True) for s in (shape, (36, 80), (36,)))
+    keep = torch.ones(*shape[:-1], 36, dtype=torch.uint8, device=DEV)
+    y = K.linear(x, w, b, act, keep, 2.0, checkpoint=True)
+    assert y.shape == (*shape[:-1], 36)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.zeros_like(y))
+    assert dx.shape == x.shape and dw.shape == w.shape and db.shape == b.shape
+    assert not dw.any() and not db.any()
