@@ -114,6 +114,8 @@ class LinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        if ctx.checkpoint:
+            _first_derivative_only('linear')
         x, scales, weight, y, mask = ctx.saved_tensors
         dz = dy.contiguous()
         if mask is not None:
@@ -384,6 +386,7 @@ class ConvBnActFn(torch.autograd.Function):
         packed = len(ctx.cfg) > 9 and ctx.cfg[9]
         held_x = None
         if ctx.checkpoint:
+            _first_derivative_only('conv_bn_act')
             held_x = Checkpoint8._of(x, x_scales)
             conv = Checkpoint8._of(conv, conv_scales).unpack()
             x = held_x.unpack() if highway else x

@@ -4,6 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+from multilingual_text_to_speech_amd import _C
 from multilingual_text_to_speech_amd import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -27,6 +28,25 @@ def test_a_forward_mode_tangent_is_refused(dual, recording):
             K.group_norm_act(t['x'], t['gamma'], t['beta'], 4, act='silu')
         with pytest.raises(RuntimeError, match='jvp'):
             K.linear(forward_ad.make_dual(w, w), w)
+
+
+def _calls(checkpoint):
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    normal = lambda *s: torch.randn(*s, generator=gen, device=DEV)  # noqa: E731
+    x, w, k, one, zero = normal(2, 9, 32), normal(8, 32), normal(8, 32, 3), torch.ones(8, device=DEV), torch.zeros(8, device=DEV)
+    return {'linear': ((x, w), lambda x, w: K.linear(x, w, checkpoint=checkpoint)),
+            'conv_bn_act': ((x, k), lambda x, w: K.conv_bn_act(x, w, one, zero, zero.clone(), one.clone(), None, kernel=3, checkpoint=checkpoint)),
+            'conv_gn_act': ((x, k), lambda x, w: K.conv_gn_act(x, w, one, zero, kernel=3, norm_groups=2, checkpoint=checkpoint))}
+
+
+@pytest.mark.parametrize('name', ['linear', 'conv_bn_act', 'conv_gn_act'])
+def test_no_second_derivative_from_a_checkpoint(name):
+    """Gradients that were asked for with create_graph=True would look like constants."""
+    leaves, f = _calls(True)[name]
+    leaves = [t.requires_grad_() for t in leaves]
+    with pytest.raises(_C.MttsError, match='second derivative'):
+        torch.autograd.grad(f(*leaves).square().sum(), leaves, create_graph=True)
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(f(*leaves).square().sum(), leaves))
 
 
 # ---- empty inputs ---------------------------------------------------------------------------------------------------------------------
