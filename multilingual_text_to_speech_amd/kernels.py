@@ -134,7 +134,7 @@ class LinearFn(torch.autograd.Function):
 def linear(x, weight, bias=None, act='identity', mask=None, mask_scale=1.0, checkpoint=False):
     """y = act(x W^T + b) [* dropout].  checkpoint=True saves x for the backward as a `Checkpoint8` (a quarter of its bytes): the weight
     gradient is the one of the 8-bit values, everything else is unchanged."""
-    return LinearFn.apply(x, weight, bias, ACT[act], mask, mask_scale, checkpoint)
+    return LinearFn.apply(x, weight, bias, ACT[act], mask, mask_scale, checkpoint and _recorded(x, weight, bias))
 
 
 # ------------------------------------------------------------------------------------------------
@@ -416,7 +416,8 @@ class ConvBnActFn(torch.autograd.Function):
 def conv_bn_act(x, weight, gamma, beta, rmean, rvar, mask, *, kernel, dilation=1, groups=1, act='identity', training=True,
                 momentum=0.1, eps=1e-5, mask_scale=1.0, highway=False, packed=False, checkpoint=False):
     """checkpoint=True saves the block's input and the convolution's output for the backward as `Checkpoint8` (a quarter of their bytes)."""
-    cfg = (kernel, dilation, groups, ACT[act], training, momentum, eps, mask_scale, highway, packed, checkpoint)
+    cfg = (kernel, dilation, groups, ACT[act], training, momentum, eps, mask_scale, highway, packed,
+           checkpoint and _recorded(x, weight, gamma, beta))
     return ConvBnActFn.apply(x, weight, gamma, beta, rmean, rvar, mask, cfg)
 
 
@@ -446,10 +447,15 @@ def _first_derivative_only(what):
         _refuse(what, 'there is no second derivative (create_graph=True)')
 
 
+def _recorded(*tensors):
+    """Whether a graph is being recorded: nobody reads what a call saves otherwise."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _differentiated(*tensors):
     """Whether autograd follows the call: a graph is being recorded, or an operand carries a forward-mode tangent (such an operand need
     not require a gradient; autograd.Function refuses it where there is no jvp)."""
-    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return _recorded(*tensors) or any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _same_device(what, device, *tensors):
@@ -771,10 +777,9 @@ def conv_gn_act(x, weight, gamma, beta, lengths=None, mask=None, *, kernel, norm
     _same_device(what, x.device, weight)
     gamma, beta, lengths, mask = _gn_check(what, (x.shape[0], x.shape[1], weight.shape[0]), x.device, gamma, beta, norm_groups, lengths, mask, act)
     require_gpu(x)
-    learns = torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, gamma, beta))
     with _On(x.device):
         lens = _device_lengths(what, lengths, x.device)
-        cfg = (kernel, dilation, groups, norm_groups, GN_ACT[act], eps, mask_scale, checkpoint and learns)
+        cfg = (kernel, dilation, groups, norm_groups, GN_ACT[act], eps, mask_scale, checkpoint and _recorded(x, weight, gamma, beta))
         return ConvGnActFn.apply(x.contiguous(), weight, gamma, beta, lens, mask, cfg)
 
 

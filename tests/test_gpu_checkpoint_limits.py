@@ -49,6 +49,20 @@ def test_no_second_derivative_from_a_checkpoint(name):
     assert all(torch.isfinite(g).all() for g in torch.autograd.grad(f(*leaves).square().sum(), leaves))
 
 
+@pytest.mark.parametrize('name', ['linear', 'conv_bn_act', 'conv_gn_act'])
+def test_nothing_is_packed_where_nothing_is_recorded(name, monkeypatch):
+    leaves, f = _calls(True)[name]
+    want = f(*[t.clone().requires_grad_() for t in leaves]).detach()
+    packs = []
+    real = K.checkpoint8
+    monkeypatch.setattr(K, 'checkpoint8', lambda *a: packs.append(a) or real(*a))
+    assert torch.equal(f(*leaves), want) and not packs                     # no operand requires a gradient
+    with torch.no_grad():
+        assert torch.equal(f(*[t.clone().requires_grad_() for t in leaves]), want) and not packs
+    f(*[t.clone().requires_grad_() for t in leaves])
+    assert packs
+
+
 # ---- empty inputs ---------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize('shape', [(0, 80), (3, 0, 80)], ids=str)
