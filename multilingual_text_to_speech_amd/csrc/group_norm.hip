@@ -786,6 +786,7 @@ static int gn_check(const GroupNormArgs& p, const char* what) {
     // a grid has fewer than 2^32 threads; strips are 32 channels wide at least, or the whole row
     MTTS_REQUIRE((long)p.N * cdiv(p.C, 32) * (p.G > cdiv(p.C, 32) ? 2 : 1) < (1L << 32) / 1024, "%s: %d samples x %d channels are too many for one call", what, p.N, p.C);
     MTTS_REQUIRE(p.C <= (1 << 24), "%s: %d channels are too many", what, p.C);
+    MTTS_REQUIRE(p.L <= 0x7fff0000, "%s: %d rows are too many for one call", what, p.L);      // a row number plus a workgroup's rows fits an int
     return 0;
 }
 

@@ -417,6 +417,7 @@ static int wg_check(const Wgrad8Args& p) {
     MTTS_REQUIRE(p.dtype == MTTS_F32 || p.dtype == MTTS_BF16, "mtts_conv_weight_grad8: dtype %d is neither MTTS_F32 nor MTTS_BF16", p.dtype);
     MTTS_REQUIRE((long)p.kernel * (p.I / p.groups) < (1L << 28) && (long)(p.kernel - 1) * p.dilation < (1L << 30), "mtts_conv_weight_grad8: kernel %d with dilation %d is too large", p.kernel, p.dilation);
     MTTS_REQUIRE(p.kernel <= 8192 && (long)p.O * (p.I / p.groups) < (1L << 32) / 256, "mtts_conv_weight_grad8: %d output x %d input channels of %d taps are too many for one call", p.O, p.I / p.groups, p.kernel);
+    MTTS_REQUIRE(p.L <= 0x7fff0000, "mtts_conv_weight_grad8: %d rows are too many for one call", p.L);      // a row number plus a step's rows fits an int
     const WgPlan k = wg_plan(p);
     MTTS_REQUIRE((long)k.tiles_m * k.tiles_n * p.groups * k.splits < (1L << 32) / 512, "mtts_conv_weight_grad8: too many tiles for one call");
     return 0;

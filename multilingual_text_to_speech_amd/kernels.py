@@ -430,11 +430,18 @@ _DTYPE = {torch.float32: 0, torch.bfloat16: 1}
 GN_ACT = {**ACT, 'silu': 4}
 
 
-_MOST_ROWS = 0x7fff0000                    # row numbers are 32-bit
+_MOST_ROWS = 0x7fff0000                    # row and channel numbers are 32-bit
 
 
 def _refuse(what, why):
     raise _C.MttsError(f'{what}: {why}')
+
+
+def _check_sizes(what, **sizes):
+    """The kernels count in 32 bits, with room for a workgroup's rows behind the last one; ctypes would cut a larger number off."""
+    for name, n in sizes.items():
+        if n > _MOST_ROWS:
+            _refuse(what, f'{n} {name} are too many for one call')
 
 
 def _check_storage(what, t, name):
@@ -546,6 +553,7 @@ class Checkpoint8:
         dtype = dtype or self.dtype
         if dtype not in _DTYPE:
             _refuse('Checkpoint8.unpack', f'dtype is {dtype}: float32 or bfloat16 is expected')
+        _check_sizes('Checkpoint8.unpack', channels=self.shape[-1])
         require_gpu(self.values)
         out = torch.empty(self.values.shape, dtype=dtype, device=self.values.device)
         if out.numel():
@@ -568,8 +576,7 @@ def checkpoint8(x, lengths=None):
         _refuse(what, f'x has shape {tuple(x.shape)}: at least one channel is expected')
     if lengths is not None:
         lengths = _check_lengths(what, lengths, x.shape[0], x.shape[1], x.device)
-    if x.numel() // x.shape[-1] > _MOST_ROWS:
-        _refuse(what, f'{x.numel() // x.shape[-1]} rows are too many for one call')
+    _check_sizes(what, rows=x.numel() // x.shape[-1], channels=x.shape[-1])
     require_gpu(x)
     if not x.is_contiguous():
         x = x.detach().contiguous()
@@ -599,8 +606,7 @@ def conv1d_weight_grad8(held, dy, kernel, dilation=1, groups=1, packed=False):
     I, O = held.shape[-1], dy.shape[-1]
     if I % groups or O % groups or not I or not O:
         _refuse(what, f'{I} x {O} channels are not a multiple of {groups} groups')
-    if dy.numel() // O > _MOST_ROWS:
-        _refuse(what, f'{dy.numel() // O} rows are too many for one call')
+    _check_sizes(what, rows=dy.numel() // O, channels=max(I, O), taps=kernel * dilation)
     require_gpu(held.values, dy)
     shape = (O, kernel, I // groups) if packed else (O, I // groups, kernel)
     rows = dy.numel() // O
@@ -689,6 +695,8 @@ class GroupNormActFn(torch.autograd.Function):
 def _gn_check(what, shape, device, gamma, beta, groups, lengths, mask, act):
     """Contiguous gamma, beta, lengths (where they are) and uint8 flags, or a refusal."""
     N, L, C = shape
+    if max(N, L, C) > _MOST_ROWS:
+        _check_sizes(what, samples=N, rows=L, channels=C)
     if groups < 1 or C < 1 or C % groups:
         _refuse(what, f'{C} channels are not a multiple of {groups} groups')
     if act not in GN_ACT:
@@ -774,6 +782,7 @@ def conv_gn_act(x, weight, gamma, beta, lengths=None, mask=None, *, kernel, norm
         _refuse(what, f'x {x.dtype} {tuple(x.shape)}, weight {weight.dtype} {tuple(weight.shape)}: float32 [N, L, I] and [O, I / groups, kernel] are expected')
     if min(kernel, dilation, groups) < 1 or not x.numel() or tuple(weight.shape[1:]) != (x.shape[2] // groups, kernel) or x.shape[2] % groups or weight.shape[0] % groups:
         _refuse(what, f'input {tuple(x.shape)} and weight {tuple(weight.shape)} do not belong to one convolution of kernel {kernel} with {groups} groups')
+    _check_sizes(what, rows=x.shape[0] * x.shape[1] + kernel * dilation)      # a tap's place among them
     _same_device(what, x.device, weight)
     gamma, beta, lengths, mask = _gn_check(what, (x.shape[0], x.shape[1], weight.shape[0]), x.device, gamma, beta, norm_groups, lengths, mask, act)
     require_gpu(x)

@@ -1,0 +1,59 @@
+"""Limits of the group norm / 8-bit checkpoint operators and the bounds of their GPU tests (no GPU needed: nothing may be launched)."""
+import ctypes
+
+import pytest
+import torch
+
+from multilingual_text_to_speech_amd import _C
+from multilingual_text_to_speech_amd import kernels as K
+
+
+@pytest.fixture(scope='module')
+def library():
+    import os
+    if not os.path.exists(_C.LIB_PATH):
+        from multilingual_text_to_speech_amd.build import build
+        build()
+    return _C.lib()
+
+
+def refused(match, f, *a, **kw):
+    with pytest.raises(_C.MttsError, match=match):
+        f(*a, **kw)
+
+
+def meta(*shape, dtype=torch.float32):
+    return torch.empty(*shape, dtype=dtype, device='meta')
+
+
+def held(*shape):
+    return K.Checkpoint8(meta(*shape, dtype=torch.int8), meta(*shape[:-1], -(-shape[-1] // 32), dtype=torch.uint8))
+
+
+@pytest.mark.parametrize('big', [2 ** 31 - 1, 2 ** 32 + 1, 2 ** 32 + 5])
+def test_sizes_that_pass_32_bits_are_refused(big):
+    """2^31 - 1 rows leave no room for a workgroup's row numbers; a C int would take 2^32 + 5 for 5."""
+    one = meta(1)
+    refused('rows are too many', K.group_norm_act, meta(1, big, 1), one, one, 1)
+    refused('samples are too many', K.group_norm_act, meta(big, 1, 1), one, one, 1)
+    refused('channels are too many', K.group_norm_act, meta(1, 1, big), meta(big), meta(big), 1)
+    refused('channels are too many', K.checkpoint8, meta(1, big))
+    refused('rows are too many', K.checkpoint8, meta(big, 1))
+    refused('channels are too many', held(1, big).unpack)
+    refused('channels are too many', K.conv1d_weight_grad8, held(1, big), meta(1, 1), 1)
+    refused('channels are too many', K.conv1d_weight_grad8, held(1, 1), meta(1, big), 1)
+    refused('taps are too many', K.conv1d_weight_grad8, held(1, 4, 1), meta(1, 4, 1), 3, dilation=big)
+    refused('taps are too many', K.conv1d_weight_grad8, held(1, 4, 1), meta(1, 4, 1), big)
+    refused('rows are too many', K.conv_gn_act, meta(1, 4, 1), meta(1, 1, 3), one, one, kernel=3, norm_groups=1, dilation=big)
+    refused('rows are too many', K.conv_gn_act, meta(1, big, 1), meta(1, 1, 3), one, one, kernel=3, norm_groups=1)
+
+
+def test_entry_points_refuse_rows_without_room(library):
+    err = lambda: library.mtts_last_error().decode()  # noqa: E731
+    a = _C.GroupNormArgs(gamma=4096, beta=4096, mean=4096, rstd=4096, ws=4096, x=4096, y=4096, dy=4096, dx=4096, N=1, L=2 ** 31 - 1, C=1, G=1)
+    for f in (library.mtts_group_norm_act_fwd, library.mtts_group_norm_act_bwd):
+        assert f(ctypes.byref(a), None) and 'rows are too many' in err()
+    assert library.mtts_group_norm_workspace_floats(ctypes.byref(a), 0) == -1
+    w = _C.Wgrad8Args(q=4096, q_code=4096, dy=4096, dw=4096, ws=4096, N=1, L=2 ** 31 - 1, I=1, O=1, kernel=1, dilation=1, groups=1)
+    assert library.mtts_conv_weight_grad8(ctypes.byref(w), None) and 'rows are too many' in err()
+    assert library.mtts_conv_weight_grad8_workspace_floats(ctypes.byref(w)) == -1
