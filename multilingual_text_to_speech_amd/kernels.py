@@ -459,10 +459,14 @@ def _recorded(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def _differentiated(*tensors):
+def _differentiated(x, gamma, beta):
     """Whether autograd follows the call: a graph is being recorded, or an operand carries a forward-mode tangent (such an operand need
     not require a gradient; autograd.Function refuses it where there is no jvp)."""
-    return _recorded(*tensors) or any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
+        return True
+    if forward_ad.unpack_dual(x).primal is x:      # outside of forward-mode differentiation: nothing has a tangent
+        return False
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in (x, gamma, beta))
 
 
 def _same_device(what, device, *tensors):
