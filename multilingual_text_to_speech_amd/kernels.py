@@ -500,7 +500,9 @@ def _check_lengths(what, lengths, N, L, device):
     if lengths is None:
         return None
     if not isinstance(lengths, torch.Tensor):
-        lengths = torch.tensor(lengths, dtype=torch.int64)
+        lengths = torch.tensor(lengths)
+        if not (lengths.numel() and lengths.is_floating_point()):            # fractions are refused below, not cut off
+            lengths = lengths.to(torch.int64)
     if tuple(lengths.shape) != (N,) or lengths.dtype not in (torch.int32, torch.int64):
         _refuse(what, f'lengths is {lengths.dtype} {tuple(lengths.shape)}: int32 or int64 of shape ({N},) is expected')
     if lengths.is_cuda:

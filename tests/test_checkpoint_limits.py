@@ -57,3 +57,16 @@ def test_entry_points_refuse_rows_without_room(library):
     w = _C.Wgrad8Args(q=4096, q_code=4096, dy=4096, dw=4096, ws=4096, N=1, L=2 ** 31 - 1, I=1, O=1, kernel=1, dilation=1, groups=1)
     assert library.mtts_conv_weight_grad8(ctypes.byref(w), None) and 'rows are too many' in err()
     assert library.mtts_conv_weight_grad8_workspace_floats(ctypes.byref(w)) == -1
+
+
+def test_lengths_that_are_no_whole_numbers_are_refused():
+    x, g = torch.zeros(2, 3, 8), torch.ones(8)
+    for lengths in ([1.5, 2.9], [1.0, 2.0], (0.5, 3)):
+        refused('int32 or int64', K.group_norm_act, x, g, g, 2, lengths)
+        refused('int32 or int64', K.checkpoint8, x, lengths)
+    refused('CPU', K.group_norm_act, x, g, g, 2, [1, 3])                      # whole ones get as far as the device
+    refused('CPU', K.group_norm_act, x, g, g, 2, (0, 3))
+    refused('CPU', K.group_norm_act, x[:0], g, g, 2, [])
+    import numpy
+    refused('CPU', K.group_norm_act, x, g, g, 2, numpy.array([1, 3]))
+    refused('CPU', K.group_norm_act, x, g, g, 2, numpy.array([1, 3], dtype=numpy.uint8))
