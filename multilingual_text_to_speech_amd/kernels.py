@@ -786,7 +786,9 @@ def conv_gn_act(x, weight, gamma, beta, lengths=None, mask=None, *, kernel, norm
     what = 'conv_gn_act'
     if x.dtype != torch.float32 or weight.dtype != torch.float32 or x.dim() != 3 or weight.dim() != 3:
         _refuse(what, f'x {x.dtype} {tuple(x.shape)}, weight {weight.dtype} {tuple(weight.shape)}: float32 [N, L, I] and [O, I / groups, kernel] are expected')
-    if min(kernel, dilation, groups) < 1 or not x.numel() or tuple(weight.shape[1:]) != (x.shape[2] // groups, kernel) or x.shape[2] % groups or weight.shape[0] % groups:
+    if not x.numel():
+        _refuse(what, f'x has shape {tuple(x.shape)}: at least one value is expected')
+    if min(kernel, dilation, groups) < 1 or tuple(weight.shape[1:]) != (x.shape[2] // groups, kernel) or x.shape[2] % groups or weight.shape[0] % groups:
         _refuse(what, f'input {tuple(x.shape)} and weight {tuple(weight.shape)} do not belong to one convolution of kernel {kernel} with {groups} groups')
     _check_sizes(what, rows=x.shape[0] * x.shape[1] + kernel * dilation)      # a tap's place among them
     _same_device(what, x.device, weight)

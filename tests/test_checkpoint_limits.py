@@ -70,3 +70,9 @@ def test_lengths_that_are_no_whole_numbers_are_refused():
     import numpy
     refused('CPU', K.group_norm_act, x, g, g, 2, numpy.array([1, 3]))
     refused('CPU', K.group_norm_act, x, g, g, 2, numpy.array([1, 3], dtype=numpy.uint8))
+
+
+def test_an_empty_block_input_is_named():
+    one = torch.ones(6)
+    for shape in ((0, 3, 8), (2, 0, 8), (2, 3, 0)):
+        refused('at least one value', K.conv_gn_act, torch.zeros(shape), torch.zeros(6, 8, 5), one, one, kernel=5, norm_groups=2)
