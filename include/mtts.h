@@ -170,7 +170,8 @@ int mtts_checkpoint8_pack(const void* x, const int* lengths, int8_t* q, uint8_t*
 int mtts_checkpoint8_unpack(const int8_t* q, const uint8_t* code, void* x, long rows, int C, int dtype, void* stream);
 
 /* ---- weight gradient of a 1-D convolution / linear layer from an 8-bit checkpoint of its input (csrc/wgrad8.hip) ----------------------
- * dw[o, c, t] = sum_{n, l} dy[n, l, o] x[n, l + t * dilation - (kernel - 1) * dilation / 2, c], zero outside [0, L), groups as F.conv1d. */
+ * dw[o, c, t] = sum_{n, l} dy[n, l, o] x[n, l + t * dilation - (kernel - 1) * dilation / 2, c], zero outside [0, L), groups as F.conv1d.
+ * An infinite fp32 dy makes its output channel's sums NaN (with one term, bf16, they are infinite or NaN as the products are). */
 typedef struct Wgrad8Args {
     const int8_t* q;       /* [N, L, I] */
     const uint8_t* q_code; /* [N, L, ceil(I / 32)] */
@@ -186,7 +187,7 @@ typedef struct Wgrad8Args {
     int groups;
     int dtype;             /* MTTS_F32 | MTTS_BF16: dy */
     int packed;
-    int precision;         /* as GemmArgs.precision: 1 rounds an fp32 dy to bf16, 2 keeps all its bits, 0 the process-wide default */
+    int precision;         /* as GemmArgs.precision: 1 rounds an fp32 dy to bf16, 2 keeps its bits down to 2^-133, 0 the process-wide default */
 } Wgrad8Args;
 
 long mtts_conv_weight_grad8_workspace_floats(const Wgrad8Args* args);      /* -1: bad arguments (mtts_last_error) */

@@ -600,8 +600,9 @@ def checkpoint8(x, lengths=None):
 def conv1d_weight_grad8(held, dy, kernel, dilation=1, groups=1, packed=False):
     """Weight gradient of a 'same'-padded 1-D convolution from the `Checkpoint8` of its input [N, L, I] and dy [N, L, O] (float32 or
     bfloat16): dW[o, c, t] = sum_{n, l} dy[n, l, o] x[n, l + t * dilation - (kernel - 1) * dilation // 2, c], float32 [O, I / groups, kernel]
-    (packed: [O, kernel, I / groups]).  kernel 1 takes inputs [..., I] of any shape: a linear layer.  A float32 dy keeps all its bits
-    unless set_precision('bf16') is on."""
+    (packed: [O, kernel, I / groups]).  kernel 1 takes inputs [..., I] of any shape: a linear layer.  A float32 dy keeps its bits down
+    to 2^-133 (all 24 from magnitudes of 2^-110 on) unless set_precision('bf16') is on; an infinity in it makes its output channel NaN.  To
+    autograd the result is a constant."""
     what = 'conv1d_weight_grad8'
     _check_storage(what, dy, 'dy')
     if kernel < 1 or dilation < 1 or groups < 1:

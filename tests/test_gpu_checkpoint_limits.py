@@ -75,3 +75,39 @@ def test_linear_of_no_rows_from_a_checkpoint(shape, act):
     dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.zeros_like(y))
     assert dx.shape == x.shape and dw.shape == w.shape and db.shape == b.shape
     assert not dw.any() and not db.any()
+
+
+# ---- limits of the weight gradient's three terms ----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('value', [float('inf'), float('-inf'), float('nan')])
+@pytest.mark.parametrize('rows', [40, 7680])                # 128- and 256-wide tiles
+def test_a_non_finite_gradient_stays_in_its_output_channel(rows, value, dtype):
+    """An infinity: NaN in three terms, the products' own infinities in one; the other channels keep their bits."""
+    O, I = (96, 64) if rows == 40 else (512, 2560)
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    held = K.checkpoint8(torch.randint(1, 100, (1, rows, I), generator=gen, device=DEV).float())
+    dy = torch.randn(1, rows, O, generator=gen, device=DEV).to(dtype)
+    clean = K.conv1d_weight_grad8(held, dy, 1)
+    dy[0, rows - 9, 17] = value
+    got = K.conv1d_weight_grad8(held, dy, 1)
+    if dtype == BF16 and value == value:
+        assert torch.equal(got[17], torch.full_like(got[17], value))          # no 8-bit value of this row is zero
+    else:
+        assert got[17].isnan().all()
+    others = torch.arange(O, device=DEV) != 17
+    assert torch.equal(got[others], clean[others]) and torch.isfinite(clean).all()
+
+
+def test_bits_of_small_gradients():
+    """One product per output, with x = 2^106.  The three terms are whole multiples of 2^-133: nothing is lost at magnitudes of 2^-110 and
+    more (24 bits), less than 2^-133 below, also where dy is subnormal; a bfloat16 dy is taken as it is."""
+    held = K.checkpoint8(torch.full((1, 1, 32), 2.0 ** 106, device=DEV))
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    for e in range(-149, -100):
+        bits = torch.randint(2 ** 23, 2 ** 24, (1, 1, 2048), generator=gen, device=DEV).double()
+        dy = (bits * 2.0 ** (e - 23)).float()
+        error = K.conv1d_weight_grad8(held, dy, 1)[:, 0, 0].double() * 2.0 ** -106 - dy.double()[0, 0]
+        assert error.abs().max() < 2.0 ** -133 and (e < -110 or not error.any())
+        half = dy.bfloat16()
+        assert torch.equal(K.conv1d_weight_grad8(held, half, 1)[:, 0, 0].double() * 2.0 ** -106, half.double()[0, 0])
