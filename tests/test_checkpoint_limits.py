@@ -6,6 +6,8 @@ import torch
 
 from multilingual_text_to_speech_amd import _C
 from multilingual_text_to_speech_amd import kernels as K
+from tests import operator_bounds as B
+from tests import operator_refs as R
 
 
 @pytest.fixture(scope='module')
@@ -76,3 +78,31 @@ def test_an_empty_block_input_is_named():
     one = torch.ones(6)
     for shape in ((0, 3, 8), (2, 0, 8), (2, 3, 0)):
         refused('at least one value', K.conv_gn_act, torch.zeros(shape), torch.zeros(6, 8, 5), one, one, kernel=5, norm_groups=2)
+
+
+# ---- the cases and bounds of the GPU tests --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('case,fp32,bf16', B.FORMS, ids=lambda v: str(v))
+def test_the_listed_shapes_reach_their_form(library, case, fp32, bf16):
+    assert (B.splits_of(case, torch.float32), B.splits_of(case, torch.bfloat16)) == (fp32, bf16)
+
+
+@pytest.mark.parametrize('kind', ['dense', 'bits', 'one'])
+def test_whole_number_cases_miss_nothing(kind):
+    """In float32 the sums are exact; a lost row, and with 17 and 24 bits a lost third plane of dy, changes them."""
+    case = (3, 50, 64, 40, 3, 2, 1)
+    v, s, dy = B.whole_numbers(case, torch.float32, kind, 1, 'cpu')
+    want = B.whole_weight_grad(v, s, dy, 3, 2, 1)
+    x = K.Checkpoint8(v, s)
+    x = x.values.float() * torch.pow(2.0, x.scales.float() - 127).repeat_interleave(32, -1)[..., :64]
+    assert torch.equal(R.weight_grad(x, dy, 3, 2, 1)[0], want) and torch.equal(want.float().double(), want)
+    one = torch.einsum('nlo,nlc->oc', dy, x)                                  # in float32
+    assert torch.equal(one.double(), want[:, :, 1])
+    for r in range(0, 50, 7):
+        lost = v.clone()
+        lost[1, r] = 0
+        assert kind == 'one' and not v[1, r].any() or not torch.equal(B.whole_weight_grad(lost, s, dy, 3, 2, 1), want)
+    if kind != 'dense':
+        a1 = (dy.view(torch.int32) & -65536).view(torch.float32)
+        a2 = ((dy - a1).view(torch.int32) & -65536).view(torch.float32)
+        assert not torch.equal(B.whole_weight_grad(v, s, a1 + a2, 3, 2, 1), want)
