@@ -106,3 +106,31 @@ def test_whole_number_cases_miss_nothing(kind):
         a1 = (dy.view(torch.int32) & -65536).view(torch.float32)
         a2 = ((dy - a1).view(torch.int32) & -65536).view(torch.float32)
         assert not torch.equal(B.whole_weight_grad(v, s, a1 + a2, 3, 2, 1), want)
+
+
+@pytest.mark.parametrize('offset', [0.0, 100.0, 3000.0])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('shape', B.LONG, ids=str)
+def test_the_bounds_of_group_norm_miss_nothing(shape, dtype, offset):
+    """The definition's own result passes; one without either mean, without one of 64 chunks in them, or with one lost in the sums for scale and
+    offset does not."""
+    if offset and dtype != torch.float32:
+        return                                    # the spread is gone in bfloat16
+    N, L, C, G = shape
+    x, gamma, beta, keep, dy, lens = B.norm_case(shape, dtype, 'tanh', 'cpu', offset=offset)
+    ref = B.norm_reference(x, gamma, beta, G, lens, keep, 'tanh', 1.0, dy, False)
+    ey, edx, edg, edb = B.norm_bounds(x, gamma, beta, G, ref, dy)
+    r = ref['rstd'].repeat_interleave(C // G, -1)[:, None, :]
+    assert not B.outside(ref['dx'].to(dtype), ref['dx'], edx).any()
+    assert not B.outside(ref['dgamma'].float(), ref['dgamma'], edg).any()
+    chunk = torch.arange(L) >= -(-L // 64)                                    # the first of 64 chunks is lost
+    m1, m2 = B.norm_means(ref, gamma, G, chunk)
+    wrong = {'m1': r * ref['m1'], 'm2': r * ref['xhat_b'] * ref['m2'], 'both': r * (ref['m1'] + ref['xhat_b'] * ref['m2'])}
+    if offset < 3000:
+        wrong['chunk'] = r * (ref['m1'] - m1 + ref['xhat_b'] * (ref['m2'] - m2))
+    for name, off in wrong.items():
+        assert B.outside((ref['dx'] + off).to(dtype), ref['dx'], edx).float().mean() > 0.05, name
+    if offset == 0:
+        for rows in (slice(L // 2, L // 2 + -(-L // 64)), slice(0, L, 100)):          # a chunk, a hundredth of the rows
+            assert B.outside((ref['dbeta'] - ref['dz'][0, rows].sum(0)).float(), ref['dbeta'], edb).float().mean() > 0.5
+            assert B.outside((ref['dgamma'] - (ref['dz'] * ref['xhat_b'])[0, rows].sum(0)).float(), ref['dgamma'], edg).float().mean() > 0.5

@@ -147,3 +147,69 @@ def test_weight_grad_of_whole_numbers_at_odd_addresses_and_in_bf16_mode(case, dt
                 assert torch.equal(K.conv1d_weight_grad8(K.Checkpoint8(vv, off(s)), dd, k, dilation=d, groups=g).double(), want)
     finally:
         _C.set_precision('fp32')
+
+
+# ---- group norm, with bounds that a missing mean, chunk or row exceeds ------------------------------------------------------------------------
+
+def close(got, want, bound, what):
+    bad = B.outside(got, want, bound)
+    assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()} values are off, the first by {(got.double() - want).abs()[bad][0].item():.3g}, bound {bound.expand_as(bad)[bad][0].item():.3g}'
+
+
+def check_norm(shape, dtype, act, ckpt, lengths, mask, offset=0.0):
+    G, scale = shape[3], 2.0 if mask else 1.0
+    x, gamma, beta, keep, dy, lens = B.norm_case(shape, dtype, act, DEV, 3, lengths, mask, offset)
+    ref = B.norm_reference(x, gamma, beta, G, lens, keep, act, scale, dy, ckpt)
+    ey, edx, edg, edb = B.norm_bounds(x, gamma, beta, G, ref, dy, scale)
+    leaves = [t.requires_grad_() for t in (x, gamma, beta)]
+    y = K.group_norm_act(*leaves, G, lens, keep, act=act, mask_scale=scale, checkpoint=ckpt)
+    dx, dgamma, dbeta = torch.autograd.grad(y, leaves, dy)
+    close(y.detach(), ref['y'], ey, 'y')
+    close(dx, ref['dx'], edx, 'dx')
+    close(dgamma, ref['dgamma'], edg, 'dgamma')
+    close(dbeta, ref['dbeta'], edb, 'dbeta')
+
+
+@pytest.mark.parametrize('ckpt', [False, True])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('shape', B.NORMS, ids=str)
+def test_every_form_of_group_norm(shape, dtype, ckpt):
+    """Ragged where there are several samples; dropout without a checkpoint."""
+    N, L = shape[:2]
+    act = ('tanh', 'silu')[B.NORMS.index(shape) % 2]
+    check_norm(shape, dtype, act, ckpt, [L, L - L // 3, 1][:N] if N > 1 else None, not ckpt)
+
+
+@pytest.mark.parametrize('offset', [100.0, 3000.0])
+@pytest.mark.parametrize('shape', [s for s in B.LONG if s[0] * s[1] * s[2] < 300000], ids=str)
+def test_group_norm_of_an_offset(shape, offset):
+    check_norm(shape, F32, 'tanh', False, None, False, offset)
+
+
+@pytest.mark.parametrize('kind', ['plain', 'highway', 'generated', 'generated highway'])
+def test_every_model_block_trains_from_checkpoints(kind, monkeypatch):
+    """activation_checkpoint_bits = 8: the same output; gradients within the rounding of the 8-bit values, 2 * 2^-7 of a block's largest value
+    in one element and far less over a tensor (bounded as in the batch norm block's test)."""
+    from multilingual_text_to_speech_amd.modules import layers as M
+    from multilingual_text_to_speech_amd.params.params import Params as hp
+    torch.manual_seed(2)
+    cls = {'plain': M.ConvBlock, 'highway': M.HighwayConvBlock, 'generated': M.ConvBlockGenerated, 'generated highway': M.HighwayConvBlockGenerated}[kind]
+    generated = 'generated' in kind
+    block = cls(*((6, 4) if generated else ()), 60, 60, 3, 0.0, 'tanh', 2, 3 if generated else 1).to(DEV)
+    x, dy = torch.randn(5, 31, 60, device=DEV), torch.randn(5, 31, 60, device=DEV)
+    e = (torch.randn(3, 6, device=DEV),) if generated else ()
+    out = {}
+    for bits in (32, 8):
+        monkeypatch.setattr(hp, 'activation_checkpoint_bits', bits, raising=False)
+        xr = x.clone().requires_grad_()
+        y = block(*e, xr)
+        out[bits] = (y.detach(), torch.autograd.grad(y, [xr, *block.parameters()], dy, allow_unused=True))
+    assert torch.equal(out[32][0], out[8][0])
+    seen = 0
+    for a, b in zip(out[8][1], out[32][1]):
+        assert (a is None) == (b is None)
+        if a is not None:
+            seen += 1
+            rel = ((a - b).norm() / b.norm()).item()
+            assert a.shape == b.shape and 0 < rel < 0.06, rel
+    assert seen >= 4
