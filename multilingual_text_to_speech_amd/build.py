@@ -16,7 +16,7 @@ OUT = os.path.join(HERE, "libmtts_hip.so")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wno-unused-result",
          "-ffp-contract=fast",
          # no v_pk_add/mul/fma_f32: hipcc makes them of ordinary float code, and some of their forms have given wrong results now and
-         # then.  (hipcc's host pass warns that it does not know the feature.)
+         # then on these cards (train step 66.9-67.0 -> 67.2-67.3 ms).  (hipcc's host pass warns that it does not know the feature.)
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 

@@ -5,8 +5,9 @@
 // (bf16) neighbouring lanes, so its maximum is three (two) DPP steps; a row's last, partial block is padded with idle lanes.  Vectors
 // start at any element and a row's last one may be partial (64 x 600 x 511 fp32, pack: 30 us element by element, 19 us so).
 //
-// 64 x 600 x 512 fp32 (98 MB each way): pack 17 us, unpack 15.4 us, 5.8 and 6.4 TB/s, with inputs that partly come from the last-level
-// cache; a copy of 1 GiB runs at 5.1 TB/s on the same card.
+// 64 x 600 x 512: fp32 (99 MB each way) pack 18.8 us, unpack 17.2 us, 5.3 and 5.8 TB/s, with inputs that partly come from the last-level
+// cache; pack with lengths from 300 to 600 (79 MB) 17 us.  bf16 (60 MB): pack 15.3 us, 3.9 TB/s (the vector instructions of the rounding),
+// unpack 10.9 us, 5.5 TB/s.  A copy of 1 GiB runs at 5.1 TB/s on the same card.
 #include "vec_io.h"
 
 constexpr int CK_T = 256;

@@ -11,7 +11,7 @@
 //
 // This is bytes: read x, write y; read x (or its checkpoint) and dy, write dx.  Two forms:
 //   * resident: one workgroup takes a sample's column strip (whole groups, at least 128 bytes wide), all rows in registers: one pass
-//     over memory, one launch each way.  Strips of up to 8192 vectors of 16 bytes (1024 rows of 128 bytes).
+//     over memory, one launch each way.  Strips of up to 8192 vectors of 16 bytes (1024 rows of 128 bytes), in the forward 12288 (1536).
 //   * two-pass: rows cut into chunks; partial moments (sums) per chunk and group, merged by every workgroup of the second pass; the
 //     second reading comes from the 256 MB last-level cache where the tensors fit.
 // Widths or addresses that no 16-byte vector fits go one value at a time, in two passes (vectors that straddle rows, with their partial
@@ -19,9 +19,10 @@
 //
 // GPU time, a copy of 1 GiB running at 5.1 TB/s on the same card (tensors below 256 MB come partly from the last-level cache):
 //   64 x 600 x 512 in 16 groups, tanh, fp32: forward with keep flags 44 us (177 MB, 4.0 TB/s), without them and over ragged samples 26 us
-//   (138 MB, 5.2 TB/s), backward with flags 51 us (256 MB, 5.0 TB/s).  bf16, silu, ragged, with the checkpoint: forward 27 us (90 MB, 3.3
-//   TB/s), backward 36 us (78 MB, 2.2 TB/s): the vector instructions of eight values to a vector.  Two passes, 4 x 4999 rows of 512, fp32,
-//   ragged, with the checkpoint: moments 17 + apply 14 us, sums 17 + apply 17 us, each about half of a copy's rate.
+//   (138 MB, 5.2 TB/s), backward with flags 51 us (256 MB, 5.0 TB/s).  bf16, silu, ragged, with the checkpoint: forward 28 us (90 MB, 3.2
+//   TB/s), backward 36 us (78 MB, 2.2 TB/s): the vector instructions of eight values to a vector, on the rows behind a length too.  Two
+//   passes, 4 x 4999 rows of 512, fp32, ragged, with the checkpoint: moments 17 us (45 MB, 2.7 TB/s) + apply 15 us (76 MB, 5.2 TB/s), sums
+//   17 us (44 MB, 2.5 TB/s) + apply 16 us (85 MB, 5.2 TB/s): the passes that reduce run at half of the rate of those that write.
 //   The sums over samples for the gradients of scale and offset: 4 us.
 #include "vec_io.h"
 
@@ -31,7 +32,7 @@ constexpr int GN_CHUNKS = 64;      // most row chunks of a sample
 
 // ---- activations ------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }      // v_rcp_f32: 1 ulp
-// tanh through exp loses digits next to zero (1 - e cancels): the odd polynomial there (its next term is 2e-9 of z at 1/4)
+// tanh through exp loses digits next to zero (1 - e cancels): the odd polynomial there (its next term is 8.5e-9 of z at 1/4)
 __device__ __forceinline__ float gn_tanh(float z) {
     const float e = __expf(-2.f * fabsf(z)), r = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), z), s = z * z;
     const float p = z + z * s * (-0.33333333333f + s * (0.13333333333f + s * (-0.05396825397f + s * 0.02186948854f)));
@@ -308,7 +309,7 @@ template <typename T, int VEC> struct GnX<T, VEC, true> {
 };
 
 // The backward keeps x as it lies in memory and dz in fp32; per-channel sums of dz and dz * xhat go to ws [2][N][C], and through gamma
-// to the two means of the group.
+// to the two means of the group.  (bf16, 16 rows, straddling vectors, no checkpoint: 13 registers spill, 56 bytes a lane.)
 template <typename T, int VEC, int R, bool STR, bool CK>
 __global__ void __launch_bounds__(512) gn_bwd_kernel(GroupNormArgs p, GnGeo k) {
     constexpr int SZ = sizeof(T), K = STR ? VEC : 1;

@@ -10,11 +10,13 @@
 // The split's limits: bits of dy worth less than 2^-133, the smallest bf16 number, are lost (magnitudes of 2^-110 and more keep all 24
 // bits), and an infinite dy makes its output channel's sums NaN (infinity minus its leading bits), where one term sums infinities.
 //
-// What bounds it: the matrix pipes.  At 38400 rows, 512 -> 512 channels, kernel 5 (100.7 GFLOP, three terms) the whole call takes 244 us,
-// 1240 TFLOP/s of bf16 products where a plain bf16 library product of 8192^3 reaches 1330 on the same card.  One term (bf16 gradients):
-// 120 us, 840 TFLOP/s: a step's 1024 cycles of matrix instructions stand beside 1024 cycles of LDS reads and writes (at 128 bytes a
-// cycle) and 900 of vector instructions, two thirds of them for the checkpoint.  At 7680 rows, bf16 (20 GFLOP) 48 us: half of that is
-// the partial tiles' way through memory (63 MB out and in at twelve splits).
+// What bounds it: the matrix pipes.  At 38400 rows, 512 -> 512 channels, kernel 5 (100.7 GFLOP, three terms) the whole call takes 235 us
+// where three of four inputs are zeros, as behind a rectifier and dropout, and 250 us where none are: 1210-1290 TFLOP/s of bf16 products
+// where a plain bf16 library product of 8192^3 reaches 1330 on the same card.  One term: bf16 gradients 116-120 us, 840-870 TFLOP/s, fp32
+// ones in bf16 mode 127-129 us: a step's 1024 cycles of matrix instructions stand beside 1024 cycles of LDS reads and writes (at 128 bytes a
+// cycle) and 900 of vector instructions, two thirds of them for the checkpoint.  At 7680 rows, bf16 (20 GFLOP) 44 us: half of that is
+// the partial tiles' way through memory (63 MB out and in at twelve splits).  Kernel 1 at 38400 rows, fp32: 67-70 us for 45 us of matrix
+// instructions, the same way for sixty-four splits of 1 MB.
 //
 // Tile TM x TN x 32 rows per workgroup, v_mfma_f32_32x32x16_bf16.  A thread takes 8 rows x 4 columns: the transposition happens in
 // registers, and 8 rows of one column are the 16 bytes that a lane feeds to the matrix instruction.  LDS holds these 16-byte units in

@@ -133,7 +133,7 @@ class LinearFn(torch.autograd.Function):
 
 def linear(x, weight, bias=None, act='identity', mask=None, mask_scale=1.0, checkpoint=False):
     """y = act(x W^T + b) [* dropout].  checkpoint=True saves x for the backward as a `Checkpoint8` (a quarter of its bytes): the weight
-    gradient is the one of the 8-bit values, everything else is unchanged."""
+    gradient is the one of the 8-bit values, everything else is unchanged (a second derivative is refused)."""
     return LinearFn.apply(x, weight, bias, ACT[act], mask, mask_scale, checkpoint and _recorded(x, weight, bias))
 
 
@@ -415,7 +415,8 @@ class ConvBnActFn(torch.autograd.Function):
 
 def conv_bn_act(x, weight, gamma, beta, rmean, rvar, mask, *, kernel, dilation=1, groups=1, act='identity', training=True,
                 momentum=0.1, eps=1e-5, mask_scale=1.0, highway=False, packed=False, checkpoint=False):
-    """checkpoint=True saves the block's input and the convolution's output for the backward as `Checkpoint8` (a quarter of their bytes)."""
+    """checkpoint=True saves the block's input and the convolution's output for the backward as `Checkpoint8` (a quarter of their bytes); a
+    second derivative is refused then."""
     cfg = (kernel, dilation, groups, ACT[act], training, momentum, eps, mask_scale, highway, packed,
            checkpoint and _recorded(x, weight, gamma, beta))
     return ConvBnActFn.apply(x, weight, gamma, beta, rmean, rvar, mask, cfg)
@@ -572,8 +573,9 @@ class Checkpoint8:
 
 def checkpoint8(x, lengths=None):
     """`Checkpoint8` of an activation [..., C] (float32 or bfloat16).  With `lengths` [N] for x [N, L, C] the rows behind a sample's length
-    are not read and stand for zeros.  The error is at most half of a step of the block's power of two (2^-7 of the block's largest
-    magnitude); magnitudes of 255/128 * 2^127 and more stop at 63/32 * 2^127."""
+    are not read and stand for zeros.  The error is at most half of a step of the block's power of two: 1/127.5 of the block's largest
+    magnitude, 2^-127 where that is below 2^-120; magnitudes of 255/128 * 2^127 and more stop at 63/32 * 2^127.  To autograd what
+    unpack() returns is a constant."""
     what = 'checkpoint8'
     _check_storage(what, x, 'x')
     if lengths is not None and x.dim() != 3:
@@ -726,7 +728,7 @@ def group_norm_act(x, gamma, beta, groups, lengths=None, mask=None, *, act='iden
     """y = dropout(act(gamma * (x - mean) / sqrt(var + eps) + beta)) over x [N, L, C] channel-last, float32 or bfloat16 (gamma, beta:
     float32).  Mean and (biased) variance of a sample's group run over its lengths[n] valid rows and the group's C / groups channels; rows
     behind the length are never read, and y and the gradient of x are zero there.  act: identity, relu, tanh, sigmoid or silu;
-    mask: uint8 keep flags [N, L, C] with the factor mask_scale, as in conv_bn_act.
+    mask: uint8 keep flags [N, L, C] with the factor mask_scale, as in conv_bn_act.  First derivatives in reverse mode only.
     checkpoint=True saves x for the backward as a `Checkpoint8`: mean and deviation stay those of x, the gradients are those of the
     8-bit values.  A backward that is captured into a graph has to be the only live graph of its leaves (torch's own rule: release the
     eager one first)."""
