@@ -615,7 +615,7 @@ def conv1d_weight_grad8(held, dy, kernel, dilation=1, groups=1, packed=False):
     I, O = held.shape[-1], dy.shape[-1]
     if I % groups or O % groups or not I or not O:
         _refuse(what, f'{I} x {O} channels are not a multiple of {groups} groups')
-    _check_sizes(what, rows=dy.numel() // O, channels=max(I, O), taps=kernel * dilation)
+    _check_sizes(what, rows=dy.numel() // O, channels=max(I, O), taps=max(kernel, (kernel - 1) * dilation))
     require_gpu(held.values, dy)
     shape = (O, kernel, I // groups) if packed else (O, I // groups, kernel)
     rows = dy.numel() // O
@@ -625,7 +625,7 @@ def conv1d_weight_grad8(held, dy, kernel, dilation=1, groups=1, packed=False):
         dy = dy.detach().contiguous()
     dw = _f32(shape, device=dy.device)
     N, L = (dy.shape[0], dy.shape[1]) if kernel > 1 else (1, rows)
-    a = _C.Wgrad8Args(held.values.data_ptr(), held.scales.data_ptr(), dy.data_ptr(), dw.data_ptr(), None, N, L, I, O, kernel, dilation, groups,
+    a = _C.Wgrad8Args(held.values.data_ptr(), held.scales.data_ptr(), dy.data_ptr(), dw.data_ptr(), None, N, L, I, O, kernel, dilation if kernel > 1 else 1, groups,
                       _DTYPE[dy.dtype], int(packed), 0)
     with _On(dy.device):
         n = lib().mtts_conv_weight_grad8_workspace_floats(ctypes.byref(a))
@@ -793,7 +793,7 @@ def conv_gn_act(x, weight, gamma, beta, lengths=None, mask=None, *, kernel, norm
         _refuse(what, f'x has shape {tuple(x.shape)}: at least one value is expected')
     if min(kernel, dilation, groups) < 1 or tuple(weight.shape[1:]) != (x.shape[2] // groups, kernel) or x.shape[2] % groups or weight.shape[0] % groups:
         _refuse(what, f'input {tuple(x.shape)} and weight {tuple(weight.shape)} do not belong to one convolution of kernel {kernel} with {groups} groups')
-    _check_sizes(what, rows=x.shape[0] * x.shape[1] + kernel * dilation)      # a tap's place among them
+    _check_sizes(what, rows=x.shape[0] * x.shape[1] + (kernel - 1) * dilation)      # a tap's place among them
     _same_device(what, x.device, weight)
     gamma, beta, lengths, mask = _gn_check(what, (x.shape[0], x.shape[1], weight.shape[0]), x.device, gamma, beta, norm_groups, lengths, mask, act)
     require_gpu(x)

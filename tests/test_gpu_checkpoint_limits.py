@@ -149,6 +149,13 @@ def test_weight_grad_of_whole_numbers_at_odd_addresses_and_in_bf16_mode(case, dt
         _C.set_precision('fp32')
 
 
+@pytest.mark.parametrize('dilation', [1 << 20, 2 ** 31 - 1, 2 ** 32, 2 ** 32 + 1])
+def test_one_tap_has_no_dilation(dilation):
+    v, s, dy = B.whole_numbers((2, 37, 64, 96, 1, 1, 1), F32, 'dense', 9, DEV)
+    got = K.conv1d_weight_grad8(K.Checkpoint8(v, s), dy, 1, dilation=dilation)
+    assert torch.equal(got.double(), B.whole_weight_grad(v, s, dy, 1, 1, 1))
+
+
 # ---- group norm, with bounds that a missing mean, chunk or row exceeds ------------------------------------------------------------------------
 
 def close(got, want, bound, what):
