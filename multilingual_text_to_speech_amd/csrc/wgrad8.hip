@@ -243,9 +243,14 @@ __global__ void __launch_bounds__((TM + TN) * KP) wgrad8_kernel(Wgrad8Args p, in
         unsigned at = base;                                              // of the next load's first row
         if constexpr (ODD && SZ == 2) {
             u32x3 r[SETS][8]; unsigned odd[SETS][8];
+            // the word that the last value shares with whatever follows the tensor: as a row behind the end it has to be zero, not a NaN
+            const unsigned end = (unsigned)(((k_end - k_begin) * p.O - first) * SZ) + lead;
             loop([&](auto set) __attribute__((always_inline)) {
 #pragma unroll
-                     for (int i = 0; i < 8; ++i) { const unsigned o = at + (unsigned)i * row; odd[set.value][i] = o & 2; r[set.value][i] = __builtin_amdgcn_raw_buffer_load_b96(rs, o & ~3u, 0, 0); }
+                     for (int i = 0; i < 8; ++i) {
+                         const unsigned o = at + (unsigned)i * row;
+                         odd[set.value][i] = o & 2; r[set.value][i] = __builtin_amdgcn_raw_buffer_load_b96(rs, o < end ? o & ~3u : 0x80000000u, 0, 0);
+                     }
                      at += BK * row;
                  },
                  [&](auto set, u32x4* to) __attribute__((always_inline)) {

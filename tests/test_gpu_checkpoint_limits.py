@@ -156,6 +156,26 @@ def test_one_tap_has_no_dilation(dilation):
     assert torch.equal(got.double(), B.whole_weight_grad(v, s, dy, 1, 1, 1))
 
 
+def among(t, poison, lead=0):
+    """t, lead elements behind an aligned address, with the poison in front of it and behind it."""
+    store = torch.full((t.numel() + 64 + lead,), poison, dtype=t.dtype, device=DEV)
+    o = store[32 + lead:32 + lead + t.numel()].view(t.shape)
+    return o.copy_(t)
+
+
+@pytest.mark.parametrize('lead', [0, 1])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('case', [(1, 7, 64, 33, 1, 1, 1), (1, 6, 81, 559, 1, 3, 1), (3, 5, 35, 33, 3, 1, 1), (5, 17, 60, 45, 3, 2, 3), (33, 301, 257, 259, 3, 2, 1),
+                                  (23, 357, 510, 511, 5, 1, 1), (41, 201, 512, 512, 5, 2, 1), (1, 9001, 40, 35, 2, 1, 1)], ids=str)
+def test_weight_grad_reads_nothing_of_its_neighbours(case, dtype, lead):
+    """NaN next to the gradient, exponents that stand for NaN next to the checkpoint's: also where a tensor ends inside a word."""
+    k, d, g = case[4:]
+    v, s, dy = B.whole_numbers(case, dtype, 'dense', 11, DEV)
+    want = B.whole_weight_grad(v, s, dy, k, d, g)
+    got = K.conv1d_weight_grad8(K.Checkpoint8(among(v, 127, lead), among(s, 255, lead)), among(dy, float('nan'), lead), k, dilation=d, groups=g)
+    assert torch.equal(got.double(), want)
+
+
 # ---- group norm, with bounds that a missing mean, chunk or row exceeds ------------------------------------------------------------------------
 
 def close(got, want, bound, what):
