@@ -1,5 +1,7 @@
 """Group norm, 8-bit checkpoints and their weight gradient on the GPU: what autograd is told, empty inputs, limits, and every form of the
 kernels with bounds close enough to miss nothing (tests/operator_bounds.py)."""
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -240,3 +242,108 @@ def test_every_model_block_trains_from_checkpoints(kind, monkeypatch):
             rel = ((a - b).norm() / b.norm()).item()
             assert a.shape == b.shape and 0 < rel < 0.06, rel
     assert seen >= 4
+
+
+# ---- neighbours in memory: nothing is read of them, nothing is written to them -------------------------------------------------------------
+
+GUARD = 64
+
+
+def hidden(*shape, dtype, lead, fill):
+    """A tensor to write to, GUARD elements of `fill` in front of it and behind it, and a check that they are still there."""
+    n = 1
+    for v in shape:
+        n *= v
+    store = torch.full((n + 2 * GUARD + lead,), fill, dtype=dtype, device=DEV)
+    view = store[GUARD + lead:GUARD + lead + n].view(shape)
+    rest = torch.ones(store.shape, dtype=torch.bool, device=DEV)
+    rest[GUARD + lead:GUARD + lead + n] = False
+
+    def untouched():
+        torch.cuda.synchronize()
+        return torch.equal(store[rest], torch.full_like(store[rest], fill))
+    return view, untouched
+
+
+# widths of whole vectors and odd ones, rows that end inside a checkpoint block, strips that cut groups, long samples
+@pytest.mark.parametrize('lead', [0, 1])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('shape', [(3, 5, 80, 8), (2, 61, 33, 3), (3, 300, 80, 8), (2, 70, 48, 2), (2, 600, 64, 4), (1, 3001, 40, 2), (1, 3001, 37, 1), (2, 17, 4100, 2), (5, 1, 7, 7)], ids=str)
+def test_group_norm_keeps_to_its_tensors(shape, dtype, lead):
+    N, L, C, G = shape
+    x, gamma, beta, keep, dy, lens = B.norm_case(shape, dtype, 'tanh', DEV, 4, [L, L - L // 3, 0, 1, 1][:N], True)
+    nan, nb = float('nan'), -(-C // 32)
+    plain = [t.clone().requires_grad_() for t in (x, gamma, beta)]
+    y = K.group_norm_act(*plain, G, lens, keep, act='tanh', mask_scale=2.0)
+    want = (y.detach(), *torch.autograd.grad(y, plain, dy))
+    held = K.checkpoint8(x, lens)
+    xs, gs, bs, ks, ds = among(x, nan, lead), among(gamma, nan, lead), among(beta, nan, lead), among(keep, 1, lead), among(dy, nan, lead)
+    outs = {'y': hidden(N, L, C, dtype=dtype, lead=lead, fill=7), 'dx': hidden(N, L, C, dtype=dtype, lead=lead, fill=7),
+            'mean': hidden(N, G, dtype=F32, lead=lead, fill=7), 'rstd': hidden(N, G, dtype=F32, lead=lead, fill=7),
+            'q': hidden(N, L, C, dtype=torch.int8, lead=lead, fill=7), 'code': hidden(N, L, nb, dtype=torch.uint8, lead=lead, fill=7),
+            'dgamma': hidden(C, dtype=F32, lead=lead, fill=7), 'dbeta': hidden(C, dtype=F32, lead=lead, fill=7)}
+    at = {k: v[0].data_ptr() for k, v in outs.items()}
+    li = among(lens.int(), 2 ** 30, lead)
+    a = _C.GroupNormArgs(xs.data_ptr(), gs.data_ptr(), bs.data_ptr(), li.data_ptr(), ks.data_ptr(), at['y'], at['mean'], at['rstd'], at['q'], at['code'], None,
+                         N, L, C, G, K._DTYPE[dtype], K.GN_ACT['tanh'], 1e-5, 2.0, ds.data_ptr(), at['dx'], at['dgamma'], at['dbeta'])
+
+    def call(entry, backward):
+        n = _C.lib().mtts_group_norm_workspace_floats(ctypes.byref(a), backward)
+        ws, intact = hidden(n, dtype=F32, lead=0, fill=7)
+        a.ws = ws.data_ptr()
+        _C.check(entry(ctypes.byref(a), _C.stream_ptr()), 'group norm')
+        assert intact() and all(u() for _, u in outs.values())
+    call(_C.lib().mtts_group_norm_act_fwd, 0)
+    if lead == 0:                                # another alignment may sum in another order
+        assert torch.equal(outs['y'][0], want[0])
+    ref = B.norm_reference(x, gamma, beta, G, lens, keep, 'tanh', 2.0, dy, False)
+    bounds = B.norm_bounds(x, gamma, beta, G, ref, dy, 2.0)
+    close(outs['y'][0], ref['y'], bounds[0], 'y')
+    assert torch.equal(outs['q'][0], held.values) and torch.equal(outs['code'][0], held.scales)
+    a.q = a.q_code = None                        # the backward from x
+    call(_C.lib().mtts_group_norm_act_bwd, 1)
+    for got, w, e in zip(('dx', 'dgamma', 'dbeta'), want[1:], bounds[1:]):
+        assert lead or torch.equal(outs[got][0], w)
+        close(outs[got][0], ref[got], e, got)
+    qs, cs = among(held.values, 127, lead), among(held.scales, 255, lead)
+    a.q, a.q_code, a.x = qs.data_ptr(), cs.data_ptr(), None
+    call(_C.lib().mtts_group_norm_act_bwd, 1)
+    ref = B.norm_reference(x, gamma, beta, G, lens, keep, 'tanh', 2.0, dy, True)
+    for got, e in zip(('dx', 'dgamma', 'dbeta'), B.norm_bounds(x, gamma, beta, G, ref, dy, 2.0)[1:]):
+        close(outs[got][0], ref[got], e, got)
+
+
+@pytest.mark.parametrize('lead', [0, 1, 3])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('shape', [(1, 1, 1), (2, 3, 33), (5, 37, 80), (3, 11, 31), (2, 100, 512), (130, 1, 39), (3, 211, 1285)], ids=str)
+def test_checkpoints_keep_to_their_tensors(shape, dtype, lead):
+    N, L, C = shape
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    x = torch.randn(*shape, generator=gen, device=DEV).to(dtype)
+    lens = torch.randint(0, L + 1, (N,), generator=gen, device=DEV, dtype=torch.int32)
+    held = K.checkpoint8(x, lens)
+    q, q_intact = hidden(*shape, dtype=torch.int8, lead=lead, fill=7)
+    code, code_intact = hidden(N, L, -(-C // 32), dtype=torch.uint8, lead=lead, fill=7)
+    back, back_intact = hidden(*shape, dtype=dtype, lead=lead, fill=7)
+    xs, li = among(x, float('nan'), lead), among(lens, 2 ** 30, lead)
+    _C.check(_C.lib().mtts_checkpoint8_pack(xs.data_ptr(), li.data_ptr(), q.data_ptr(), code.data_ptr(), N, L, C, K._DTYPE[dtype], _C.stream_ptr()), 'pack')
+    _C.check(_C.lib().mtts_checkpoint8_unpack(q.data_ptr(), code.data_ptr(), back.data_ptr(), N * L, C, K._DTYPE[dtype], _C.stream_ptr()), 'unpack')
+    assert q_intact() and code_intact() and back_intact()
+    assert torch.equal(q, held.values) and torch.equal(code, held.scales) and torch.equal(back, held.unpack())
+
+
+@pytest.mark.parametrize('packed', [0, 1])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('case', [(1, 7, 64, 33, 1, 1, 1), (5, 17, 60, 45, 3, 2, 3), (33, 301, 257, 259, 3, 2, 1), (23, 357, 510, 511, 5, 1, 1), (64, 120, 512, 512, 5, 1, 1),
+                                  (64, 600, 32, 64, 3, 1, 1), (2, 400, 8, 8, 2500, 1, 1)], ids=str)
+def test_weight_grad_keeps_to_its_tensors(case, dtype, packed):
+    N, L, I, O, k, d, g = case
+    v, s, dy = B.whole_numbers(case, dtype, 'dense', 13, DEV)
+    want = B.whole_weight_grad(v, s, dy, k, d, g)
+    dw, intact = hidden(*((O, k, I // g) if packed else (O, I // g, k)), dtype=F32, lead=1, fill=7)
+    a = _C.Wgrad8Args(v.data_ptr(), s.data_ptr(), dy.data_ptr(), dw.data_ptr(), None, N, L, I, O, k, d, g, K._DTYPE[dtype], packed, 0)
+    ws, ws_intact = hidden(_C.lib().mtts_conv_weight_grad8_workspace_floats(ctypes.byref(a)), dtype=F32, lead=0, fill=7)
+    a.ws = ws.data_ptr()
+    _C.check(_C.lib().mtts_conv_weight_grad8(ctypes.byref(a), _C.stream_ptr()), 'weight gradient')
+    assert intact() and ws_intact()
+    assert torch.equal((dw.permute(0, 2, 1) if packed else dw).double(), want)
