@@ -347,3 +347,31 @@ def test_weight_grad_keeps_to_its_tensors(case, dtype, packed):
     _C.check(_C.lib().mtts_conv_weight_grad8(ctypes.byref(a), _C.stream_ptr()), 'weight gradient')
     assert intact() and ws_intact()
     assert torch.equal((dw.permute(0, 2, 1) if packed else dw).double(), want)
+
+
+@pytest.mark.parametrize('name', ['linear', 'conv_bn_act', 'conv_gn_act'])
+def test_blocks_from_checkpoints_captured_and_replayed(name):
+    """Forward and backward in one graph, replayed with eager work between: the eager bits each time."""
+    (x, w), f = _calls(True)[name]
+
+    def step(a, b):
+        leaves = [a.detach().requires_grad_(), b.detach().requires_grad_()]
+        y = f(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, torch.ones_like(y))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, w)
+    gen = torch.Generator(device=DEV).manual_seed(14)
+    for _ in range(4):
+        x.copy_(torch.randn(x.shape, generator=gen, device=DEV))
+        w.copy_(torch.randn(w.shape, generator=gen, device=DEV))
+        want = step(x, w)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert all(torch.equal(a, b) for a, b in zip(step(x, w), want))
